@@ -22,7 +22,7 @@ import numpy as np
 
 from . import _build
 
-__all__ = ["Engine", "Sampler", "Batch", "SamplerError", "make_params", "PARAMS_DTYPE", "load_library", "library_path",
+__all__ = ["Engine", "Sampler", "Batch", "Head", "SamplerError", "make_params", "PARAMS_DTYPE", "load_library", "library_path",
            "LOGITS_ON_HOST", "WRITE_BACK", "KEEP_KEPT_SET", "MAX_CANDIDATE_K", "API_SYMBOLS"]
 
 LOGITS_ON_HOST = 1
@@ -52,10 +52,14 @@ API_SYMBOLS = [
     "fsb_stream_state_get", "fsb_stream_state_set", "fsb_sample_batch", "fsb_verify_windows", "fsb_last_kept",
     "fsb_batch_prepare", "fsb_batch_redraw", "fsb_batch_launch", "fsb_batch_tokens", "fsb_batch_kernel_count",
     "fsb_batch_free", "fsb_counters",
+    "fsb_stream_penalties_set", "fsb_stream_bias_set", "fsb_adjust_logits", "fsb_sample_batch_adjusted",
+    "fsb_head_create", "fsb_head_free", "fsb_head_logits", "fsb_sample_hidden",
 ]
 
 STATUS_NAMES = {0: "FSB_OK", -1: "FSB_ERR_INVALID", -2: "FSB_ERR_RANGE", -3: "FSB_ERR_CAPACITY", -4: "FSB_ERR_CUDA",
-                -5: "FSB_ERR_STREAM_ID", -6: "FSB_ERR_NO_DEVICE", -7: "FSB_ERR_DEVICE"}
+                -5: "FSB_ERR_STREAM_ID", -6: "FSB_ERR_NO_DEVICE", -7: "FSB_ERR_DEVICE", -8: "FSB_ERR_EMPTY"}
+ELEMENT_TYPES = {"float32": 0, "bfloat16": 1, "float16": 2}   # FSB_F32, FSB_BF16, FSB_F16
+WEIGHTS_ON_HOST = 1
 
 
 class SamplerError(RuntimeError):
@@ -137,6 +141,14 @@ def load_library(build_if_missing: bool = True):
     L.fsb_stream_history_append.argtypes = [vp, i32, vp, i32]
     L.fsb_stream_history_len.argtypes = [vp, i32, C.POINTER(i64)]
     L.fsb_sample_batch_resident.argtypes = [vp, i32, vp, vp, i64, i32, vp, u32]
+    L.fsb_stream_penalties_set.argtypes = [vp, i32, C.c_float, C.c_float]
+    L.fsb_stream_bias_set.argtypes = [vp, i32, vp, vp, i32]
+    L.fsb_adjust_logits.argtypes = [vp, i32, vp, vp, i32, i64, i32, vp, i64, i32, vp, vp, i32, i64]
+    L.fsb_sample_batch_adjusted.argtypes = [vp, i32, vp, vp, i32, i64, i32, vp, i64, i32, vp, vp, u32]
+    L.fsb_head_create.argtypes = [vp, i32, i32, i32, vp, vp, i32, u32, C.POINTER(vp)]
+    L.fsb_head_free.argtypes = [vp, vp]
+    L.fsb_head_logits.argtypes = [vp, vp, i32, vp, i32, i64, vp, i64]
+    L.fsb_sample_hidden.argtypes = [vp, vp, i32, vp, vp, i32, i64, vp, i64, i32, vp, vp, u32]
     L.fsb_argmax_rows_static.argtypes = [C.c_int, vp, i64, i32, i32, vp, vp, u32]
     for name in API_SYMBOLS:
         if name not in ("fsb_last_error", "fsb_params_default", "fsb_server_defaults_init", "fsb_batch_tokens_device"):
@@ -181,6 +193,38 @@ def _logits_pointer(logits, n_vocab, flags):
         ld = logits.stride(0) if logits.dim() == 2 else n_vocab
         return int(logits.data_ptr()), int(ld), flags & ~LOGITS_ON_HOST, logits
     raise TypeError("logits: numpy array or device tensor expected")
+
+
+def _device_rows(t, device: int, what: str):
+    """A two-dimensional device tensor (rows contiguous): its address, element type and row stride."""
+    kind = ELEMENT_TYPES.get(str(t.dtype).rsplit(".", 1)[-1])
+    if kind is None:
+        raise TypeError(f"{what}: {t.dtype} is not one of {', '.join(ELEMENT_TYPES)}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: a matrix with contiguous rows is expected")
+    _check_device(t, device, what)
+    return int(t.data_ptr()), kind, int(t.stride(0)) if t.shape[0] > 1 else max(int(t.stride(0)), int(t.shape[1]))
+
+
+def _check_device(t, device: int, what: str):
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{what} is on {t.device}, the engine on cuda:{device}")
+
+
+def _mask_words(masks, device: int):
+    """Packed masks (a two-dimensional 32-bit integer device tensor, or None): address, row stride, number."""
+    if masks is None:
+        return 0, 0, 0
+    if str(masks.dtype) not in ("torch.int32", "torch.uint32"):
+        raise TypeError(f"masks: {masks.dtype} is not a 32-bit integer type")
+    if masks.dim() != 2 or (masks.shape[1] > 1 and masks.stride(1) != 1):
+        raise ValueError("masks: a matrix of words with contiguous rows is expected")
+    _check_device(masks, device, "masks")
+    # (one row alone may have any stride: what lies in it is what counts)
+    ld = int(masks.shape[1]) if masks.shape[0] <= 1 else int(masks.stride(0))
+    if ld < masks.shape[1]:
+        raise ValueError("masks: rows overlap")
+    return int(masks.data_ptr()), ld, int(masks.shape[0])
 
 
 class Batch:
@@ -247,6 +291,37 @@ class Batch:
             self._ptr, self._pv = None, 0
 
 
+class Head:
+    """An LM head with 4-bit weights (``fsb_head_create``; made by ``Engine.load_head``): hidden states to logits."""
+
+    def __init__(self, engine: "Engine", ptr, n_vocab: int, n_hidden: int):
+        self.engine, self._ptr, self.n_vocab, self.n_hidden = engine, ptr, n_vocab, n_hidden
+
+    def logits(self, hidden, out):
+        """``out`` [rows][n_vocab] float32 = the logits of ``hidden`` [rows][n_hidden] bfloat16 / float16; both device tensors.
+        Asynchronous on the engine's stream; returns ``out``."""
+        e = self.engine
+        hp, ht, hld = e._hidden_rows(self, hidden)
+        op, ot, old = _device_rows(out, e.device, "out")
+        if ot != ELEMENT_TYPES["float32"] or tuple(out.shape) != (hidden.shape[0], self.n_vocab):
+            raise ValueError(f"out: float32 of shape ({hidden.shape[0]}, {self.n_vocab}) is expected")
+        rc = _native.head_logits(e._hv, self._ptr or 0, int(hidden.shape[0]), hp, ht, hld, op, old)
+        if rc:
+            e._check(rc)
+        return out
+
+    def free(self):
+        if self._ptr and self.engine._h:   # (an engine that is closed has freed its heads)
+            self.engine._check(self.engine.lib.fsb_head_free(self.engine._h, self._ptr))
+        self._ptr = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class Engine:
     """One sampler engine on one CUDA device."""
 
@@ -258,7 +333,7 @@ class Engine:
             raise SamplerError(rc, "fsb_create failed (a CUDA device of compute capability 10.x is required; there is no CPU path)")
         self._h = h
         self._hv = h.value   # the same handle as an integer, for the native calls
-        self.max_rows, self.max_vocab = max_rows, max_vocab
+        self.max_rows, self.max_vocab, self.device = max_rows, max_vocab, device
 
     # -- plumbing
     def _check(self, rc: int):
@@ -388,6 +463,91 @@ class Engine:
         else:
             ptr, ld = int(logits), (n_vocab if ld is None else ld)
         out = _native.sample_batch_resident(self._hv, stream_ids, ptr, ld, n_vocab, flags)
+        if type(out) is int:
+            self._check(out)
+        return out
+
+    # ---- in front of the sampler (fsb_adjust_logits, fsb_head_*): see the C header for what is computed
+    def set_penalties(self, stream_id: int, frequency: float = 0.0, presence: float = 0.0):
+        """Frequency and presence penalty of a stream, over the window of its repetition penalty."""
+        self._check(self.lib.fsb_stream_penalties_set(self._h, int(stream_id), float(frequency), float(presence)))
+
+    def set_bias(self, stream_id: int, ids, values=None):
+        """Logit biases of a stream: a dict {token id: bias}, or ids and values.  Replaces what was set before."""
+        if values is None:
+            ids, values = list(ids.keys()), list(ids.values())
+        ids, values = np.ascontiguousarray(ids, dtype=np.int32).ravel(), np.ascontiguousarray(values, dtype=np.float32).ravel()
+        if len(ids) != len(values):
+            raise ValueError("one value per id is expected")
+        self._check(self.lib.fsb_stream_bias_set(self._h, int(stream_id), ids.ctypes.data, values.ctypes.data, len(ids)))
+
+    def _logits_rows(self, stream_ids, logits, n_vocab):
+        p, t, ld = _device_rows(logits, self.device, "logits")
+        if logits.shape[0] != len(stream_ids):
+            raise ValueError(f"{logits.shape[0]} rows for {len(stream_ids)} streams")
+        n_vocab = int(logits.shape[1]) if n_vocab is None else int(n_vocab)
+        if not 0 < n_vocab <= logits.shape[1]:
+            raise ValueError(f"n_vocab {n_vocab} is not between 1 and the rows' {logits.shape[1]}")
+        return p, t, ld, n_vocab
+
+    def _hidden_rows(self, head, hidden):
+        if not isinstance(head, Head) or head.engine is not self:
+            raise ValueError("not a head of this engine")
+        if hidden.dim() != 2 or hidden.shape[1] != head.n_hidden:
+            raise ValueError(f"hidden: a matrix of {head.n_hidden} columns is expected")
+        return _device_rows(hidden, self.device, "hidden")
+
+    def adjust_logits(self, stream_ids, logits, out, masks=None, mask_rows=None, n_vocab: int | None = None):
+        """Penalties, biases and masks (``fsb_adjust_logits``): ``logits`` [rows][n_vocab] float32 / bfloat16 / float16 into ``out``
+        (float32 or the same type; may be ``logits``), both device tensors.  masks: [n][words] int32 device tensor, bit v % 32 of
+        word v / 32 allows token v; mask_rows: the mask of every row, -1 for none.  Asynchronous on the engine's stream; returns ``out``."""
+        p, t, ld, n_vocab = self._logits_rows(stream_ids, logits, n_vocab)
+        op, ot, old = _device_rows(out, self.device, "out")
+        if out.shape[0] != logits.shape[0] or out.shape[1] < n_vocab:
+            raise ValueError(f"out: shape ({logits.shape[0]}, {n_vocab}) is expected")
+        mp, mld, mn = _mask_words(masks, self.device)
+        rc = _native.adjust_logits(self._hv, stream_ids, p, t, ld, n_vocab, mp, mld, mn, mask_rows, op, ot, old)
+        if rc:
+            self._check(rc)
+        return out
+
+    def sample_batch_adjusted(self, stream_ids, logits, masks=None, mask_rows=None, n_vocab: int | None = None, flags: int = 0) -> np.ndarray:
+        """``sample_batch_resident`` over adjusted logits (``fsb_sample_batch_adjusted``); the caller's logits stay as they are."""
+        p, t, ld, n_vocab = self._logits_rows(stream_ids, logits, n_vocab)
+        mp, mld, mn = _mask_words(masks, self.device)
+        out = _native.sample_adjusted(self._hv, stream_ids, p, t, ld, n_vocab, mp, mld, mn, mask_rows, flags)
+        if type(out) is int:
+            self._check(out)
+        return out
+
+    def load_head(self, weights, scales) -> Head:
+        """An LM head (``fsb_head_create``): weights [n_vocab][n_hidden / 2] uint8, two 4-bit weights to a byte (the first in the low
+        bits, value q - 8), scales [n_vocab][n_hidden / group] float16 / bfloat16; tensors on the engine's device or the host."""
+        kind = ELEMENT_TYPES.get(str(scales.dtype).rsplit(".", 1)[-1])
+        if str(weights.dtype) != "torch.uint8" or kind not in (1, 2):
+            raise TypeError("weights are uint8, scales float16 or bfloat16")
+        if weights.dim() != 2 or scales.dim() != 2 or weights.shape[0] != scales.shape[0] or not weights.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("weights and scales: contiguous matrices with one row per token are expected")
+        n_vocab, n_hidden = int(weights.shape[0]), 2 * int(weights.shape[1])
+        if scales.shape[1] == 0 or n_hidden % scales.shape[1]:
+            raise ValueError(f"{scales.shape[1]} scales do not divide {n_hidden} weights into groups")
+        if weights.device != scales.device:
+            raise ValueError("weights and scales are on different devices")
+        on_host = weights.device.type == "cpu"
+        if not on_host:
+            _check_device(weights, self.device, "weights")
+        ptr = C.c_void_p()
+        self._check(self.lib.fsb_head_create(self._h, n_vocab, n_hidden, n_hidden // int(scales.shape[1]), int(weights.data_ptr()), int(scales.data_ptr()), kind,
+                                             WEIGHTS_ON_HOST if on_host else 0, C.byref(ptr)))
+        return Head(self, ptr.value, n_vocab, n_hidden)
+
+    def sample_hidden(self, head: Head, stream_ids, hidden, masks=None, mask_rows=None, flags: int = 0) -> np.ndarray:
+        """A decode step from hidden states to tokens (``fsb_sample_hidden``)."""
+        p, t, ld = self._hidden_rows(head, hidden)
+        if hidden.shape[0] != len(stream_ids):
+            raise ValueError(f"{hidden.shape[0]} rows for {len(stream_ids)} streams")
+        mp, mld, mn = _mask_words(masks, self.device)
+        out = _native.sample_hidden(self._hv, stream_ids, p, t, ld, head._ptr or 0, mp, mld, mn, mask_rows, flags)
         if type(out) is int:
             self._check(out)
         return out

@@ -1,0 +1,172 @@
+// fsb_engine.h - the engine as the host files see it: streams, batches, the handle, and the steps of a call that they share.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <random>
+#include <string>
+#include <vector>
+
+#include "../../include/ferro_sampler_b200.h"
+#include "fsb_internal.h"
+
+namespace fsb {
+
+struct Stream {
+    ferro_sampler_params p{};
+    std::mt19937_64 rng;
+    uint64_t seed_used = 0;
+    uint64_t draws = 0;
+    bool open = false;
+    // device-resident history (optional): a host mirror, and a region [pool_off, pool_off + 2^pool_class) of the
+    // engine's id pool that holds its first dev_len ids
+    std::vector<int32_t> hist;
+    int64_t pool_off = -1;
+    int pool_class = -1;
+    int64_t dev_len = 0;
+    uint64_t seen = 0;   // number of the last call that listed this stream (a stream may appear once per call)
+    // what the request asks of its logits beside the repetition penalty (fsb_adjust_logits); the biases - n ids in
+    // ascending order, then their n values - in a region of the id pool of their own
+    float frequency = 0.0f, presence = 0.0f;
+    int64_t bias_off = -1;
+    int bias_class = -1;
+    int n_bias = 0;
+};
+
+}  // namespace fsb
+
+struct fsb_batch {
+    int n_rows = 0, n_vocab = 0;
+    int64_t ld = 0;
+    unsigned flags = 0;
+    int cap_rows = 0;
+    int64_t cap_hist = 0;
+    int n_cand = 0, n_full = 0;   // rows of the candidate kernel / of the full-row kernel
+    int kmax = 1;
+    fsb::SelectPlan plan;         // how the streaming kernel is laid out
+    bool all_greedy = false;      // every row of the streaming kernel is greedy
+    int window_max = 0;           // ids of the longest penalty window
+    bool penalised = false;       // some row of the streaming kernel has a penalty window
+    int64_t hist_ids = 0;         // window ids staged with the batch
+    bool sent_with_launch = false;   // descriptors and staged ids are arguments of the launch, the device copy is stale
+    int64_t gather_ids = 0;       // window values a write-back for a host caller brings back
+    int64_t table_ints = 0;       // int32 words of the per-stream table of a resident verification call, staged behind the window ids
+    // pinned host staging: [RowDesc x cap_rows][int32 x cap_hist], tokens, gathered window values
+    unsigned char* h_in = nullptr;
+    int32_t* h_tokens = nullptr;
+    int32_t* h_tokens_dev = nullptr;   // the device's address of h_tokens (pinned memory is mapped): kernels mirror tokens and a status flag there
+    bool mirrored = false;            // the last launch wrote the mirror: tokens need no copy back
+    float* h_patched = nullptr;
+    float* h_patched_dev = nullptr;    // the device's address of h_patched
+    // device
+    unsigned char* d_in = nullptr;
+    int32_t* d_tokens = nullptr;
+    float* d_patched = nullptr;
+    std::vector<int> sid;
+    std::vector<unsigned char> stochastic;
+    std::vector<fsb::RowDesc> descs;   // descriptors in row order while a batch is staged (capacity kept between calls)
+    bool launched = false;
+    // Prepared batches: a redraw's copy reads h_in when its turn comes.  `ev_sent` is recorded behind it, but not for callers
+    // that were seen to wait for every step (it costs 3 us a step: 512 x 32768 sharded 72 -> 75).
+    bool sending = false;        // the copy may not have run yet
+    bool queues_steps = true;    // the caller does not wait for every step, as far as is known
+    bool redrawn = false;
+    cudaEvent_t ev_sent = nullptr;
+    const int32_t* hist_dev = nullptr;   // where the rows' penalty windows live: the batch's staged copy, or the engine's id pool
+
+    fsb::RowDesc* h_rows() const { return reinterpret_cast<fsb::RowDesc*>(h_in); }
+    int32_t* h_hist() const { return reinterpret_cast<int32_t*>(h_in + sizeof(fsb::RowDesc) * (size_t)cap_rows); }
+    fsb::RowDesc* d_rows() const { return reinterpret_cast<fsb::RowDesc*>(d_in); }
+    int32_t* d_hist() const { return reinterpret_cast<int32_t*>(d_in + sizeof(fsb::RowDesc) * (size_t)cap_rows); }
+    // the kernels' status word sits right behind the tokens, so that one copy brings both back
+    uint32_t* d_status() const { return reinterpret_cast<uint32_t*>(d_tokens + cap_rows); }
+    size_t in_bytes_used() const { return sizeof(fsb::RowDesc) * (size_t)cap_rows + sizeof(int32_t) * (size_t)(hist_ids + table_ints); }
+};
+
+// An LM head on the device, its weights laid out once (fsb_head.cu).
+struct fsb_head {
+    int n_vocab = 0, n_hidden = 0, group = 0, scale_type = 0;
+    unsigned char* d_weights = nullptr;
+    unsigned char* d_scales = nullptr;
+};
+
+struct fsb_handle {
+    int device = 0;
+    int max_rows = 0, max_vocab = 0;
+    int64_t max_hist = 0;
+    int sm_count = 0;
+    cudaStream_t stream = nullptr;
+    bool own_stream = false;
+    cudaStream_t side = nullptr;       // the full-vocabulary kernel of a mixed batch runs here, beside the streaming kernel
+    cudaEvent_t ev_fork = nullptr, ev_join = nullptr;
+    float softcap = 0.0f;
+    int32_t vocab_offset = 0;
+    int32_t global_vocab = 0;          // vocabulary sharding: columns of the whole row (0: this engine holds whole rows)
+    int launch_overlap = 0;
+    uint64_t call_no = 0;              // counts the calls that check their streams for duplicates
+    std::vector<fsb::Stream> streams;
+    std::vector<int> free_ids;
+    // device scratch shared by all batches of this handle
+    int32_t* d_kept_ids = nullptr;
+    double* d_kept_pr = nullptr;
+    int32_t* d_kept_n = nullptr;
+    bool kept_valid = false;
+    // prompt-lookup drafting: descriptors up, drafts stored into pinned memory by the kernel
+    fsb::LookupDesc* h_lookup = nullptr;
+    fsb::LookupDesc* d_lookup = nullptr;
+    int32_t* h_drafts = nullptr;
+    int32_t* h_drafts_dev = nullptr;   // the device's address of h_drafts
+    float* d_logits_stage = nullptr;   // device copy of host logits: max_rows x max_vocab, allocated with the engine
+    size_t logits_stage_elems = 0;
+    float* h_logits = nullptr;         // pinned memory through which a few host rows go to the device
+    int32_t* h_ids = nullptr;          // ring through which new history ids go to the device without waiting
+    size_t h_ids_pos = 0;
+    uint64_t* d_trace = nullptr;       // caller-owned diagnostics buffer, or null
+    fsb_batch* own = nullptr;          // the batch behind fsb_sample_batch / fsb_verify_windows
+    int32_t* d_pool = nullptr;         // resident histories: max_hist ids, carved into power-of-two regions
+    int64_t pool_top = 0;              // ids handed out so far (bump pointer)
+    std::vector<std::vector<int64_t>> pool_free;   // freed regions by size class
+    // adjusted steps: per row how many CTAs are done, with a bit for a logit that is left (zero between calls), and a pinned
+    // word that tells of a row without one
+    uint32_t* d_row_state = nullptr;
+    uint32_t* h_empty = nullptr;
+    uint32_t* h_empty_dev = nullptr;
+    std::vector<fsb_head*> heads;      // LM heads, freed with the engine at the latest
+    fsb_counters_t counters{};
+    std::string err;
+};
+
+namespace fsb {
+
+int fail(fsb_handle* h, int code, const char* fmt, ...);
+
+#define FSB_CUDA(h, call)                                                                                       \
+    do {                                                                                                        \
+        cudaError_t e_ = (call);                                                                                \
+        if (e_ != cudaSuccess) return fsb::fail(h, FSB_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));      \
+    } while (0)
+
+bool is_greedy(const ferro_sampler_params& p);
+bool is_capturing(const fsb_handle* h);
+Stream* get_stream(fsb_handle* h, int sid);
+// First position of the penalty window of a history of `len` ids (src/sampler.cpp:11-14), whatever the penalties are.
+int64_t window_start(const ferro_sampler_params& p, int64_t len);
+int check_common(fsb_handle* h, int n_rows, int64_t ld, int n_vocab, const fsb_batch* b);
+
+// Regions of the id pool: 2^cls ids, cls >= 8.
+int take_region(fsb_handle* h, int64_t need, int64_t* off, int* cls);
+void give_region(fsb_handle* h, int64_t off, int cls);
+int ensure_region(fsb_handle* h, Stream* s, int64_t need);
+int sync_history(fsb_handle* h, Stream* s);
+// Queues a copy of host ids (pageable memory that may change after return) into the id pool.
+int upload_ids(fsb_handle* h, int64_t pool_off, const int32_t* ids, size_t count);
+
+void fill_desc(const fsb_handle* h, RowDesc& d, const ferro_sampler_params& p, int n_vocab, int64_t logits_off, int64_t hist_begin, int64_t hist_len,
+               uint64_t word, int out_index);
+int finalize_batch(fsb_handle* h, fsb_batch* b);
+int run_staged(fsb_handle* h, fsb_batch* b, const float* logits, unsigned flags, int32_t* tokens_out, int window_append = 0);
+void rollback_draws(fsb_handle* h, const fsb_batch* b);
+void count_rows(fsb_handle* h, const fsb_batch* b);
+void release_head(fsb_head* head);   // device memory and the object itself
+
+}  // namespace fsb

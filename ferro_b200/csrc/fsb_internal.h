@@ -134,6 +134,53 @@ int launch_full_row_kernel(const float* logits, const RowDesc* rows, int n_rows,
                            int32_t* kept_ids, double* kept_pr, int32_t* kept_n, int record, uint32_t* status, uint32_t* status_host, int n_vocab,
                            int vocab_offset, int write_back, float softcap, uint64_t* trace, void* stream);
 
+// ---- in front of the sampler ---------------------------------------------------------------------------------
+// What one row's logits go through (fsb_adjust.cu).
+struct AdjustRow {
+    int64_t hist_begin;    // first id of the penalty window in the id pool
+    int64_t bias_begin;    // n_bias ids in ascending order, then as many values, in the id pool
+    int32_t hist_len;
+    int32_t n_bias;
+    float repetition, frequency, presence;
+    int32_t mask_row;      // row of the mask array, or -1
+};
+static_assert(sizeof(AdjustRow) == 40, "AdjustRow layout");
+
+struct AdjustArgs {
+    const void* in;            // [rows][ld]
+    void* out;                 // [rows][out_ld]; may be `in`
+    const int32_t* pool;       // id pool
+    const uint32_t* masks;     // [.][mask_ld] words; bit id % 32 of word id / 32 allows token id
+    uint32_t* row_state;       // null, or per row the number of CTAs done (zero between launches); then `empty` is set ...
+    uint32_t* empty;           // ... (a pinned host word: 1 + the row) if a row has no logit left above minus infinity
+    int64_t ld, out_ld, mask_ld;
+    int32_t in_type, out_type; // FSB_F32, FSB_BF16, FSB_F16
+    int32_t n_rows, n_vocab;
+    int32_t first_row;         // the call's number of row 0
+    int32_t vocab_offset;      // token id of column 0
+    float softcap;             // 0 = off
+};
+// Launches for n_rows rows; rows_host is read before the call returns.  Returns a cudaError_t as int.
+int launch_adjust(const AdjustArgs& a, const AdjustRow* rows_host, void* stream, int* launches);
+
+// The head's device layout (fsb_head.cu): bytes of weights and scales, and the kernel that brings them into it.
+int64_t head_weight_bytes(int n_vocab, int n_hidden);
+int64_t head_scale_bytes(int n_vocab, int n_hidden, int group);
+int launch_head_layout(const unsigned char* weights, const void* scales, int n_vocab, int n_hidden, int group, unsigned char* weights_out,
+                       unsigned char* scales_out, void* stream);
+struct HeadArgs {
+    const unsigned char* weights;
+    const unsigned char* scales;
+    const void* hidden;        // [rows][ld_hidden]
+    float* logits;             // [rows][ld]
+    int64_t ld_hidden, ld;
+    int32_t n_rows, n_vocab, n_hidden, group;
+    int32_t scale_type, hidden_type;
+    int32_t sms;
+};
+int prepare_head_kernels();   // for the current device, before its first launch_head
+int launch_head(const HeadArgs& a, void* stream, int* launches);
+
 }  // namespace fsb
 
 // fsb_sample_batch and fsb_verify_windows with one history array per row / stream instead of a packed one; for the

@@ -1,0 +1,455 @@
+// fsb_logits.cpp - host side of what stands in front of the sampler: stream penalties and biases, logit adjustment, the LM
+// head, and the calls that go through them to tokens.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "fsb_engine.h"
+
+using namespace fsb;
+
+namespace {
+
+// No exception leaves the C ABI: the vectors of a call may find no memory.
+template <class F>
+int guarded(fsb_handle* h, F&& f) {
+    try {
+        return f();
+    } catch (...) {
+        h->err = "no host memory";   // (short enough to need none itself)
+        return FSB_ERR_INVALID;
+    }
+}
+
+size_t type_size(int type) { return type == FSB_F32 ? 4 : 2; }
+
+struct Masks {
+    const uint32_t* bits;
+    int64_t ld;
+    int n;
+    const int32_t* rows;
+};
+
+int check_masks(fsb_handle* h, const Masks& m, int n_rows, int n_vocab) {
+    if (!m.bits) {
+        if (m.rows)
+            for (int i = 0; i < n_rows; ++i)
+                if (m.rows[i] != -1) return fail(h, FSB_ERR_INVALID, "row %d has mask %d, and there are no masks", i, m.rows[i]);
+        return FSB_OK;
+    }
+    if (reinterpret_cast<uintptr_t>(m.bits) % 4) return fail(h, FSB_ERR_INVALID, "masks are not aligned to 4 bytes");
+    if (m.ld < ((int64_t)h->vocab_offset + n_vocab + 31) / 32)
+        return fail(h, FSB_ERR_INVALID, "mask rows of %lld words do not cover %lld token ids", (long long)m.ld, (long long)h->vocab_offset + n_vocab);
+    if (!m.rows && m.n < n_rows) return fail(h, FSB_ERR_INVALID, "%d masks for %d rows", m.n, n_rows);
+    if (m.rows)
+        for (int i = 0; i < n_rows; ++i)
+            if (m.rows[i] < -1 || m.rows[i] >= m.n) return fail(h, FSB_ERR_INVALID, "row %d has mask %d of %d", i, m.rows[i], m.n);
+    return FSB_OK;
+}
+
+int check_rows(fsb_handle* h, const void* p, int type, int64_t ld, int n_vocab, const char* what) {
+    if (!p) return fail(h, FSB_ERR_INVALID, "%s is null", what);
+    if (type != FSB_F32 && type != FSB_BF16 && type != FSB_F16) return fail(h, FSB_ERR_INVALID, "%s: unknown element type %d", what, type);
+    if (ld < n_vocab) return fail(h, FSB_ERR_INVALID, "%s: row stride %lld is smaller than %d", what, (long long)ld, n_vocab);
+    if (reinterpret_cast<uintptr_t>(p) % type_size(type)) return fail(h, FSB_ERR_INVALID, "%s is not aligned to its elements", what);
+    return FSB_OK;
+}
+
+// Whether two matrices' address ranges intersect.
+bool overlap(const void* a, int64_t ld_a, int cols_a, size_t size_a, const void* b, int64_t ld_b, int cols_b, size_t size_b, int rows) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t a1 = a0 + ((size_t)(rows - 1) * (size_t)ld_a + (size_t)cols_a) * size_a, b1 = b0 + ((size_t)(rows - 1) * (size_t)ld_b + (size_t)cols_b) * size_b;
+    return a0 < b1 && b0 < a1;
+}
+
+// The streams of a call: all open, and (`once`) each listed at most once.
+int check_streams(fsb_handle* h, int n_rows, const int* stream_ids, bool once) {
+    if (!stream_ids) return fail(h, FSB_ERR_INVALID, "stream_ids is null");
+    ++h->call_no;
+    for (int i = 0; i < n_rows; ++i) {
+        Stream* s = get_stream(h, stream_ids[i]);
+        if (!s) return fail(h, FSB_ERR_STREAM_ID, "row %d: unknown stream id %d", i, stream_ids[i]);
+        if (once && s->seen == h->call_no) return fail(h, FSB_ERR_INVALID, "stream %d appears twice in one resident batch", stream_ids[i]);
+        s->seen = h->call_no;
+    }
+    return FSB_OK;
+}
+
+// Queues the adjustment of rows whose arguments have been checked and whose histories are on the device.
+int queue_adjust(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab, const Masks& m, void* out,
+                 int out_type, int64_t out_ld, bool report_empty) {
+    std::vector<AdjustRow> rows((size_t)n_rows);
+    for (int i = 0; i < n_rows; ++i) {
+        const Stream* s = get_stream(h, stream_ids[i]);
+        AdjustRow& r = rows[(size_t)i];
+        const int64_t len = (int64_t)s->hist.size();
+        const bool penalties = s->p.repetition_penalty != 1.0f || s->frequency != 0.0f || s->presence != 0.0f;
+        const int64_t from = penalties ? window_start(s->p, len) : len;
+        r.hist_begin = std::max<int64_t>(s->pool_off, 0) + from;
+        r.hist_len = (int32_t)(len - from);
+        r.bias_begin = std::max<int64_t>(s->bias_off, 0);
+        r.n_bias = s->n_bias;
+        r.repetition = s->p.repetition_penalty;
+        r.frequency = s->frequency;
+        r.presence = s->presence;
+        r.mask_row = !m.bits ? -1 : m.rows ? m.rows[i] : i;
+    }
+    AdjustArgs a{};
+    a.in = logits;
+    a.out = out;
+    a.pool = h->d_pool;
+    a.masks = m.bits;
+    a.row_state = report_empty ? h->d_row_state : nullptr;
+    a.empty = h->h_empty_dev;
+    a.ld = ld;
+    a.out_ld = out_ld;
+    a.mask_ld = m.ld;
+    a.in_type = logits_type;
+    a.out_type = out_type;
+    a.n_rows = n_rows;
+    a.n_vocab = n_vocab;
+    a.vocab_offset = h->vocab_offset;
+    a.softcap = h->softcap;
+    int launches = 0;
+    const int e = launch_adjust(a, rows.data(), h->stream, &launches);
+    h->counters.kernel_launches += (uint64_t)launches;
+    if (e != 0) return fail(h, FSB_ERR_CUDA, "adjust kernel launch: %s", cudaGetErrorString((cudaError_t)e));
+    return FSB_OK;
+}
+
+// While rows that the kernel before has just written are sampled: no reads before it is complete, and (`capped`) no second
+// softcap.
+struct FreshRows {
+    fsb_handle* h;
+    const float softcap;
+    const int overlap;
+    FreshRows(fsb_handle* h_, bool capped) : h(h_), softcap(h_->softcap), overlap(h_->launch_overlap) {
+        if (capped) h->softcap = 0.0f;
+        if (overlap == 1) h->launch_overlap = 2;
+    }
+    ~FreshRows() {
+        h->softcap = softcap;
+        h->launch_overlap = overlap;
+    }
+};
+
+// Rows in the engine's memory start on 16-byte boundaries where there is room for that.
+int64_t stage_ld(const fsb_handle* h, int n_rows, int n_vocab) {
+    const int64_t ld = ((int64_t)n_vocab + 3) / 4 * 4;
+    return (size_t)n_rows * (size_t)ld <= h->logits_stage_elems ? ld : n_vocab;
+}
+
+// Adjusts `logits` into the engine's staging area and samples there.  The arguments have been checked.
+int sample_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab, const Masks& m,
+                    int32_t* tokens_out, unsigned flags) {
+    fsb_batch* b = h->own;
+    const bool append = (flags & FSB_APPEND_SAMPLED) != 0;
+    for (int i = 0; i < n_rows; ++i) {
+        Stream* s = get_stream(h, stream_ids[i]);
+        int rc = sync_history(h, s);
+        if (rc == FSB_OK && append) rc = ensure_region(h, s, (int64_t)s->hist.size() + 1);
+        if (rc) return rc;
+    }
+    const int64_t sld = stage_ld(h, n_rows, n_vocab);
+    volatile uint32_t* empty = h->h_empty;
+    *empty = 0u;
+    int rc = queue_adjust(h, n_rows, stream_ids, logits, logits_type, ld, n_vocab, m, h->d_logits_stage, FSB_F32, sld, true);
+    if (rc) return rc;
+    b->n_rows = n_rows;
+    b->n_vocab = n_vocab;
+    b->ld = sld;
+    b->flags = flags & ~FSB_APPEND_SAMPLED;
+    b->hist_dev = h->d_pool;
+    b->hist_ids = 0;
+    b->table_ints = 0;
+    b->gather_ids = 0;
+    b->sid.assign(stream_ids, stream_ids + n_rows);
+    b->stochastic.assign((size_t)n_rows, 0);
+    b->descs.resize((size_t)n_rows);
+    for (int i = 0; i < n_rows; ++i) {
+        Stream* s = get_stream(h, stream_ids[i]);
+        uint64_t word = 0;
+        if (!is_greedy(s->p)) {
+            word = s->rng();
+            s->draws++;
+            b->stochastic[(size_t)i] = 1;
+        }
+        // an empty window that ends where the history does: an appended token goes there
+        fill_desc(h, b->descs[(size_t)i], s->p, n_vocab, (int64_t)i * sld, std::max<int64_t>(s->pool_off, 0) + (int64_t)s->hist.size(), 0, word, i);
+        if (append) b->descs[(size_t)i].flags |= kRowAppend;
+    }
+    rc = finalize_batch(h, b);
+    if (rc) {
+        rollback_draws(h, b);
+        return rc;
+    }
+    {
+        FreshRows fresh(h, true);
+        rc = run_staged(h, b, h->d_logits_stage, flags & ~FSB_APPEND_SAMPLED, nullptr);
+    }
+    if (*empty != 0u) {
+        if (rc == FSB_OK) {
+            cudaStreamSynchronize(h->stream);
+            rollback_draws(h, b);
+        }
+        h->kept_valid = false;
+        return fail(h, FSB_ERR_EMPTY, "masks and biases leave row %u no token", *empty - 1u);
+    }
+    if (rc) return rc;
+    for (int i = 0; i < n_rows; ++i) {
+        tokens_out[i] = b->h_tokens[i];
+        if (append) {   // the device copy already holds the token
+            Stream* s = get_stream(h, stream_ids[i]);
+            s->hist.push_back(tokens_out[i]);
+            s->dev_len = (int64_t)s->hist.size();
+        }
+    }
+    count_rows(h, b);
+    return FSB_OK;
+}
+
+int check_sampling(fsb_handle* h, const int32_t* tokens_out, unsigned flags) {
+    if (!tokens_out) return fail(h, FSB_ERR_INVALID, "tokens_out is null");
+    if (flags & ~(FSB_APPEND_SAMPLED | FSB_KEEP_KEPT_SET)) return fail(h, FSB_ERR_INVALID, "flags 0x%x are not defined for this call", flags);
+    if (h->global_vocab > 0) return fail(h, FSB_ERR_INVALID, "a vocabulary shard's rows are not sampled alone");
+    if (is_capturing(h)) return fail(h, FSB_ERR_INVALID, "the call waits for its tokens: not inside a stream capture");
+    return FSB_OK;
+}
+
+bool owns(const fsb_handle* h, const fsb_head* head) { return head && std::find(h->heads.begin(), h->heads.end(), head) != h->heads.end(); }
+
+int check_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidden, int hidden_type, int64_t ld_hidden) {
+    if (!owns(h, head)) return fail(h, FSB_ERR_INVALID, "not a head of this engine");
+    if (n_rows <= 0) return fail(h, FSB_ERR_INVALID, "n_rows must be positive");
+    if (n_rows > 65535) return fail(h, FSB_ERR_CAPACITY, "%d rows in one call, at most 65535", n_rows);
+    if (hidden_type == FSB_F32) return fail(h, FSB_ERR_INVALID, "hidden states are FSB_BF16 or FSB_F16");
+    return check_rows(h, hidden, hidden_type, ld_hidden, head->n_hidden, "hidden");
+}
+
+int queue_head(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidden, int hidden_type, int64_t ld_hidden, float* logits, int64_t ld) {
+    HeadArgs a{};
+    a.weights = head->d_weights;
+    a.scales = head->d_scales;
+    a.hidden = hidden;
+    a.logits = logits;
+    a.ld_hidden = ld_hidden;
+    a.ld = ld;
+    a.n_rows = n_rows;
+    a.n_vocab = head->n_vocab;
+    a.n_hidden = head->n_hidden;
+    a.group = head->group;
+    a.scale_type = head->scale_type;
+    a.hidden_type = hidden_type;
+    a.sms = h->sm_count;
+    int launches = 0;
+    const int e = launch_head(a, h->stream, &launches);
+    h->counters.kernel_launches += (uint64_t)launches;
+    if (e != 0) return fail(h, FSB_ERR_CUDA, "head kernel launch: %s", cudaGetErrorString((cudaError_t)e));
+    return FSB_OK;
+}
+
+int create_head(fsb_handle* h, int n_vocab, int n_hidden, int group, const uint8_t* weights, const void* scales, int scale_type, unsigned flags,
+                fsb_head** out) {
+    if (!weights || !scales) return fail(h, FSB_ERR_INVALID, "null weights or scales");
+    if (n_vocab <= 0 || n_vocab > (1 << 20)) return fail(h, FSB_ERR_CAPACITY, "n_vocab %d is not between 1 and %d", n_vocab, 1 << 20);
+    if (group != 32 && group != 64 && group != 128) return fail(h, FSB_ERR_RANGE, "groups of %d weights: 32, 64 or 128 are supported", group);
+    if (n_hidden <= 0 || n_hidden % group || n_hidden > FSB_MAX_HIDDEN)
+        return fail(h, FSB_ERR_RANGE, "n_hidden %d is not a multiple of %d up to %d", n_hidden, group, FSB_MAX_HIDDEN);
+    if (scale_type != FSB_BF16 && scale_type != FSB_F16) return fail(h, FSB_ERR_INVALID, "scales are FSB_BF16 or FSB_F16");
+    if (reinterpret_cast<uintptr_t>(scales) % 2) return fail(h, FSB_ERR_INVALID, "scales are not aligned to their elements");
+    if (flags & ~FSB_WEIGHTS_ON_HOST) return fail(h, FSB_ERR_INVALID, "flags 0x%x are not defined for this call", flags);
+    if (is_capturing(h)) return fail(h, FSB_ERR_INVALID, "a head is not created inside a stream capture");
+    const int prepared = prepare_head_kernels();
+    if (prepared != 0) return fail(h, FSB_ERR_CUDA, "head kernels: %s", cudaGetErrorString((cudaError_t)prepared));
+    h->heads.reserve(h->heads.size() + 1);
+    fsb_head* head = new fsb_head();
+    head->n_vocab = n_vocab;
+    head->n_hidden = n_hidden;
+    head->group = group;
+    head->scale_type = scale_type;
+    const size_t wb = (size_t)n_vocab * (size_t)(n_hidden / 2), sb = (size_t)n_vocab * (size_t)(n_hidden / group) * 2;
+    unsigned char *tmp_w = nullptr, *tmp_s = nullptr;
+    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&head->d_weights), (size_t)head_weight_bytes(n_vocab, n_hidden));
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&head->d_scales), (size_t)head_scale_bytes(n_vocab, n_hidden, group));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();   // whatever stream the weights were written on
+    if (e == cudaSuccess && (flags & FSB_WEIGHTS_ON_HOST)) {
+        e = cudaMalloc(reinterpret_cast<void**>(&tmp_w), wb);
+        if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&tmp_s), sb);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(tmp_w, weights, wb, cudaMemcpyHostToDevice, h->stream);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(tmp_s, scales, sb, cudaMemcpyHostToDevice, h->stream);
+        weights = tmp_w;
+        scales = tmp_s;
+    }
+    if (e == cudaSuccess)
+        e = (cudaError_t)launch_head_layout(weights, scales, n_vocab, n_hidden, group, head->d_weights, head->d_scales, h->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(h->stream);
+    if (tmp_w) cudaFree(tmp_w);
+    if (tmp_s) cudaFree(tmp_s);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        release_head(head);
+        return fail(h, FSB_ERR_CUDA, "head creation: %s", cudaGetErrorString(e));
+    }
+    h->heads.push_back(head);
+    h->counters.kernel_launches++;
+    *out = head;
+    return FSB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fsb_stream_penalties_set(fsb_handle* h, int stream_id, float frequency, float presence) {
+    if (!h) return FSB_ERR_INVALID;
+    Stream* s = get_stream(h, stream_id);
+    if (!s) return fail(h, FSB_ERR_STREAM_ID, "unknown stream id %d", stream_id);
+    if (!std::isfinite(frequency) || !std::isfinite(presence)) return fail(h, FSB_ERR_RANGE, "penalties must be finite");
+    s->frequency = frequency;
+    s->presence = presence;
+    return FSB_OK;
+}
+
+int fsb_stream_bias_set(fsb_handle* h, int stream_id, const int32_t* ids, const float* values, int n) {
+    if (!h) return FSB_ERR_INVALID;
+    return guarded(h, [&]() -> int {
+        Stream* s = get_stream(h, stream_id);
+        if (!s) return fail(h, FSB_ERR_STREAM_ID, "unknown stream id %d", stream_id);
+        if (n < 0 || (n > 0 && (!ids || !values))) return fail(h, FSB_ERR_INVALID, "bad bias list");
+        if (is_capturing(h)) return fail(h, FSB_ERR_INVALID, "biases are not set inside a stream capture");
+        std::vector<std::pair<int32_t, float>> list((size_t)n);
+        for (int i = 0; i < n; ++i) {
+            if (!(values[i] < INFINITY)) return fail(h, FSB_ERR_RANGE, "the bias of token %d is neither finite nor minus infinity", ids[i]);
+            list[(size_t)i] = {ids[i], values[i]};
+        }
+        std::sort(list.begin(), list.end());
+        for (int i = 1; i < n; ++i)
+            if (list[(size_t)i].first == list[(size_t)i - 1].first) return fail(h, FSB_ERR_INVALID, "token %d is biased twice", list[(size_t)i].first);
+        std::vector<int32_t> words(2 * (size_t)n);
+        for (int i = 0; i < n; ++i) {
+            words[(size_t)i] = list[(size_t)i].first;
+            std::memcpy(&words[(size_t)n + (size_t)i], &list[(size_t)i].second, sizeof(float));
+        }
+        cudaSetDevice(h->device);
+        int64_t off = s->bias_off;
+        int cls = s->bias_class;
+        const bool fits = off >= 0 && 2 * (int64_t)n <= ((int64_t)1 << cls);
+        int rc = FSB_OK;
+        if (n > 0 && !fits) rc = take_region(h, 2 * (int64_t)n, &off, &cls);
+        if (rc == FSB_OK && n > 0) {
+            rc = upload_ids(h, off, words.data(), words.size());
+            if (rc && !fits) give_region(h, off, cls);
+        }
+        if (rc) return rc;
+        if (n == 0 || !fits) give_region(h, s->bias_off, s->bias_class);
+        s->bias_off = n > 0 ? off : -1;
+        s->bias_class = n > 0 ? cls : -1;
+        s->n_bias = n;
+        return FSB_OK;
+    });
+}
+
+int fsb_adjust_logits(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab, const uint32_t* masks,
+                      int64_t mask_ld, int n_masks, const int32_t* mask_rows, void* out, int out_type, int64_t out_ld) {
+    if (!h) return FSB_ERR_INVALID;
+    return guarded(h, [&]() -> int {
+        const Masks m{masks, mask_ld, n_masks, mask_rows};
+        int rc = check_common(h, n_rows, ld, n_vocab, h->own);
+        if (rc == FSB_OK) rc = check_rows(h, logits, logits_type, ld, n_vocab, "logits");
+        if (rc == FSB_OK) rc = check_rows(h, out, out_type, out_ld, n_vocab, "out");
+        if (rc == FSB_OK && out_type != FSB_F32 && out_type != logits_type)
+            rc = fail(h, FSB_ERR_INVALID, "adjusted logits are fp32 or of the logits' own type");
+        const bool in_place = out == logits && out_type == logits_type && out_ld == ld;
+        if (rc == FSB_OK && !in_place && overlap(logits, ld, n_vocab, type_size(logits_type), out, out_ld, n_vocab, type_size(out_type), n_rows))
+            rc = fail(h, FSB_ERR_INVALID, "out overlaps the logits");
+        if (rc == FSB_OK) rc = check_masks(h, m, n_rows, n_vocab);
+        if (rc == FSB_OK) rc = check_streams(h, n_rows, stream_ids, false);
+        if (rc) return rc;
+        cudaSetDevice(h->device);
+        if (is_capturing(h)) return fail(h, FSB_ERR_INVALID, "a replay would see the histories of the capture: not inside a stream capture");
+        for (int i = 0; i < n_rows && rc == FSB_OK; ++i) rc = sync_history(h, get_stream(h, stream_ids[i]));
+        if (rc) return rc;
+        return queue_adjust(h, n_rows, stream_ids, logits, logits_type, ld, n_vocab, m, out, out_type, out_ld, false);
+    });
+}
+
+int fsb_sample_batch_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab,
+                              const uint32_t* masks, int64_t mask_ld, int n_masks, const int32_t* mask_rows, int32_t* tokens_out, unsigned flags) {
+    if (!h) return FSB_ERR_INVALID;
+    return guarded(h, [&]() -> int {
+        const Masks m{masks, mask_ld, n_masks, mask_rows};
+        cudaSetDevice(h->device);
+        int rc = check_common(h, n_rows, ld, n_vocab, h->own);
+        if (rc == FSB_OK) rc = check_rows(h, logits, logits_type, ld, n_vocab, "logits");
+        if (rc == FSB_OK) rc = check_masks(h, m, n_rows, n_vocab);
+        if (rc == FSB_OK) rc = check_streams(h, n_rows, stream_ids, true);
+        if (rc == FSB_OK) rc = check_sampling(h, tokens_out, flags);
+        if (rc) return rc;
+        return sample_adjusted(h, n_rows, stream_ids, logits, logits_type, ld, n_vocab, m, tokens_out, flags);
+    });
+}
+
+int fsb_head_create(fsb_handle* h, int n_vocab, int n_hidden, int group, const uint8_t* weights, const void* scales, int scale_type, unsigned flags,
+                    fsb_head** out) {
+    if (!h) return FSB_ERR_INVALID;
+    if (!out) return fail(h, FSB_ERR_INVALID, "null argument");
+    *out = nullptr;
+    return guarded(h, [&]() -> int {
+        cudaSetDevice(h->device);
+        return create_head(h, n_vocab, n_hidden, group, weights, scales, scale_type, flags, out);
+    });
+}
+
+int fsb_head_free(fsb_handle* h, fsb_head* head) {
+    if (!h) return FSB_ERR_INVALID;
+    if (!owns(h, head)) return fail(h, FSB_ERR_INVALID, "not a head of this engine");
+    cudaSetDevice(h->device);
+    cudaStreamSynchronize(h->stream);
+    h->heads.erase(std::find(h->heads.begin(), h->heads.end(), head));
+    release_head(head);
+    return FSB_OK;
+}
+
+int fsb_head_logits(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidden, int hidden_type, int64_t ld_hidden, float* logits, int64_t ld) {
+    if (!h) return FSB_ERR_INVALID;
+    int rc = check_hidden(h, head, n_rows, hidden, hidden_type, ld_hidden);
+    if (rc == FSB_OK) rc = check_rows(h, logits, FSB_F32, ld, head->n_vocab, "logits");
+    if (rc == FSB_OK && overlap(hidden, ld_hidden, head->n_hidden, 2, logits, ld, head->n_vocab, 4, n_rows)) rc = fail(h, FSB_ERR_INVALID, "logits overlap the hidden states");
+    if (rc) return rc;
+    cudaSetDevice(h->device);
+    return queue_head(h, head, n_rows, hidden, hidden_type, ld_hidden, logits, ld);
+}
+
+int fsb_sample_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const int* stream_ids, const void* hidden, int hidden_type, int64_t ld_hidden,
+                      const uint32_t* masks, int64_t mask_ld, int n_masks, const int32_t* mask_rows, int32_t* tokens_out, unsigned flags) {
+    if (!h) return FSB_ERR_INVALID;
+    return guarded(h, [&]() -> int {
+        const Masks m{masks, mask_ld, n_masks, mask_rows};
+        cudaSetDevice(h->device);
+        int rc = check_hidden(h, head, n_rows, hidden, hidden_type, ld_hidden);
+        if (rc == FSB_OK) rc = check_common(h, n_rows, head->n_vocab, head->n_vocab, h->own);
+        if (rc == FSB_OK) rc = check_masks(h, m, n_rows, head->n_vocab);
+        if (rc == FSB_OK) rc = check_streams(h, n_rows, stream_ids, true);
+        if (rc == FSB_OK) rc = check_sampling(h, tokens_out, flags);
+        if (rc) return rc;
+        const int V = head->n_vocab;
+        const int64_t ld = stage_ld(h, n_rows, V);
+        rc = queue_head(h, head, n_rows, hidden, hidden_type, ld_hidden, h->d_logits_stage, ld);
+        if (rc) return rc;
+        bool adjusted = masks != nullptr;
+        for (int i = 0; i < n_rows && !adjusted; ++i) {
+            const Stream* s = get_stream(h, stream_ids[i]);
+            adjusted = s->frequency != 0.0f || s->presence != 0.0f || s->n_bias > 0;
+        }
+        if (adjusted) return sample_adjusted(h, n_rows, stream_ids, h->d_logits_stage, FSB_F32, ld, V, m, tokens_out, flags);
+        // nothing that the sampling kernels do not know: they apply the repetition penalty and the softcap themselves
+        FreshRows fresh(h, false);
+        return fsb_sample_batch_resident(h, n_rows, stream_ids, h->d_logits_stage, ld, V, tokens_out, flags);
+    });
+}
+
+}  // extern "C"

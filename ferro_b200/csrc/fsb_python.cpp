@@ -323,7 +323,97 @@ PyObject* batch_merge_launch_packed(PyObject*, PyObject* args) {
     return PyLong_FromLong(rc);
 }
 
+// None or one mask row per row, as adjust_logits and its like take it.  False with an exception set on failure.
+bool take_mask_rows(PyObject* o, npy_intp n, Refs& refs, const int32_t** out) {
+    *out = nullptr;
+    if (o == Py_None) return true;
+    PyArrayObject* a = refs.keep(as_i32(o));
+    if (!a) return false;
+    if (PyArray_SIZE(a) != n) {
+        PyErr_SetString(PyExc_ValueError, "one mask row per row is expected");
+        return false;
+    }
+    *out = i32(a);
+    return true;
+}
+const uint32_t* words(unsigned long long p) { return reinterpret_cast<const uint32_t*>((uintptr_t)p); }
+
+// adjust_logits(handle, stream_ids, logits pointer, type, ld, n_vocab, masks pointer, mask ld, masks, mask_rows or None, out pointer, type, ld) -> status
+PyObject* adjust_logits(PyObject*, PyObject* args) {
+    unsigned long long h, logits, masks, out;
+    long long ld, mask_ld, out_ld;
+    int type, n_vocab, n_masks, out_type;
+    PyObject *sids_o, *mr_o;
+    if (!PyArg_ParseTuple(args, "KOKiLiKLiOKiL", &h, &sids_o, &logits, &type, &ld, &n_vocab, &masks, &mask_ld, &n_masks, &mr_o, &out, &out_type, &out_ld))
+        return nullptr;
+    Refs refs;
+    PyArrayObject* sids = refs.keep(as_i32(sids_o));
+    if (!sids) return nullptr;
+    const npy_intp n = PyArray_SIZE(sids);
+    const int32_t* mask_rows;
+    if (!take_mask_rows(mr_o, n, refs, &mask_rows)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fsb_adjust_logits(handle(h), (int)n, i32(sids), reinterpret_cast<const void*>((uintptr_t)logits), type, ld, n_vocab, words(masks), mask_ld, n_masks,
+                           mask_rows, reinterpret_cast<void*>((uintptr_t)out), out_type, out_ld);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+// sample_adjusted(handle, stream_ids, logits pointer, type, ld, n_vocab, masks pointer, mask ld, masks, mask_rows or None, flags) -> tokens
+// sample_hidden(handle, stream_ids, hidden pointer, type, ld, head, masks pointer, mask ld, masks, mask_rows or None, flags) -> tokens
+PyObject* sample_through(PyObject* args, bool hidden) {
+    unsigned long long h, rows, masks, head_or_vocab;
+    long long ld, mask_ld;
+    int type, n_masks;
+    unsigned flags;
+    PyObject *sids_o, *mr_o;
+    if (!PyArg_ParseTuple(args, "KOKiLKKLiOI", &h, &sids_o, &rows, &type, &ld, &head_or_vocab, &masks, &mask_ld, &n_masks, &mr_o, &flags)) return nullptr;
+    Refs refs;
+    PyArrayObject* sids = refs.keep(as_i32(sids_o));
+    if (!sids) return nullptr;
+    const npy_intp n = PyArray_SIZE(sids);
+    const int32_t* mask_rows;
+    if (!take_mask_rows(mr_o, n, refs, &mask_rows)) return nullptr;
+    PyArrayObject* tokens = refs.keep(new_i32(n));
+    if (!tokens) return nullptr;
+    std::memset(i32(tokens), 0, sizeof(int32_t) * (size_t)n);
+    const void* p = reinterpret_cast<const void*>((uintptr_t)rows);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    if (hidden)
+        rc = fsb_sample_hidden(handle(h), reinterpret_cast<const fsb_head*>((uintptr_t)head_or_vocab), (int)n, i32(sids), p, type, ld, words(masks), mask_ld,
+                               n_masks, mask_rows, i32(tokens), flags);
+    else
+        rc = fsb_sample_batch_adjusted(handle(h), (int)n, i32(sids), p, type, ld, (int)head_or_vocab, words(masks), mask_ld, n_masks, mask_rows, i32(tokens),
+                                       flags);
+    Py_END_ALLOW_THREADS
+    if (rc) return PyLong_FromLong(rc);
+    Py_INCREF(tokens);
+    return reinterpret_cast<PyObject*>(tokens);
+}
+PyObject* sample_adjusted(PyObject*, PyObject* args) { return sample_through(args, false); }
+PyObject* sample_hidden(PyObject*, PyObject* args) { return sample_through(args, true); }
+
+// head_logits(handle, head, rows, hidden pointer, type, ld, logits pointer, ld) -> status
+PyObject* head_logits(PyObject*, PyObject* args) {
+    unsigned long long h, head, hidden, logits;
+    long long ld_hidden, ld;
+    int n_rows, type;
+    if (!PyArg_ParseTuple(args, "KKiKiLKL", &h, &head, &n_rows, &hidden, &type, &ld_hidden, &logits, &ld)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fsb_head_logits(handle(h), reinterpret_cast<const fsb_head*>((uintptr_t)head), n_rows, reinterpret_cast<const void*>((uintptr_t)hidden), type, ld_hidden,
+                         reinterpret_cast<float*>((uintptr_t)logits), ld);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 PyMethodDef methods[] = {
+    {"adjust_logits", adjust_logits, METH_VARARGS, nullptr},
+    {"sample_adjusted", sample_adjusted, METH_VARARGS, nullptr},
+    {"sample_hidden", sample_hidden, METH_VARARGS, nullptr},
+    {"head_logits", head_logits, METH_VARARGS, nullptr},
     {"sample_batch", sample_batch, METH_VARARGS, nullptr},
     {"sample_batch_resident", sample_batch_resident, METH_VARARGS, nullptr},
     {"verify_windows", verify_windows, METH_VARARGS, nullptr},

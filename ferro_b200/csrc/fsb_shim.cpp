@@ -19,121 +19,13 @@
 #include <string>
 #include <vector>
 
-#include "../../include/ferro_sampler_b200.h"
-#include "fsb_internal.h"
+#include "fsb_engine.h"
 
 static_assert(sizeof(ferro_sampler_params) == 40, "parameter struct must match the reference's 40-byte SamplerParams");
 static_assert(offsetof(ferro_sampler_params, seed) == 32, "seed sits at offset 32 in the reference struct");
 static_assert(FSB_MAX_CANDIDATE_K == fsb::kMaxK, "header constant out of step with the kernel geometry");
 
-namespace {
-
-struct Stream {
-    ferro_sampler_params p{};
-    std::mt19937_64 rng;
-    uint64_t seed_used = 0;
-    uint64_t draws = 0;
-    bool open = false;
-    // device-resident history (optional): a host mirror, and a region [pool_off, pool_off + 2^pool_class) of the
-    // engine's id pool that holds its first dev_len ids
-    std::vector<int32_t> hist;
-    int64_t pool_off = -1;
-    int pool_class = -1;
-    int64_t dev_len = 0;
-    uint64_t seen = 0;   // number of the last call that listed this stream (a stream may appear once per call)
-};
-
-}  // namespace
-
-struct fsb_batch {
-    int n_rows = 0, n_vocab = 0;
-    int64_t ld = 0;
-    unsigned flags = 0;
-    int cap_rows = 0;
-    int64_t cap_hist = 0;
-    int n_cand = 0, n_full = 0;   // rows of the candidate kernel / of the full-row kernel
-    int kmax = 1;
-    fsb::SelectPlan plan;         // how the streaming kernel is laid out
-    bool all_greedy = false;      // every row of the streaming kernel is greedy
-    int window_max = 0;           // ids of the longest penalty window
-    bool penalised = false;       // some row of the streaming kernel has a penalty window
-    int64_t hist_ids = 0;         // window ids staged with the batch
-    bool sent_with_launch = false;   // descriptors and staged ids are arguments of the launch, the device copy is stale
-    int64_t gather_ids = 0;       // window values a write-back for a host caller brings back
-    int64_t table_ints = 0;       // int32 words of the per-stream table of a resident verification call, staged behind the window ids
-    // pinned host staging: [RowDesc x cap_rows][int32 x cap_hist], tokens, gathered window values
-    unsigned char* h_in = nullptr;
-    int32_t* h_tokens = nullptr;
-    int32_t* h_tokens_dev = nullptr;   // the device's address of h_tokens (pinned memory is mapped): kernels mirror tokens and a status flag there
-    bool mirrored = false;            // the last launch wrote the mirror: tokens need no copy back
-    float* h_patched = nullptr;
-    float* h_patched_dev = nullptr;    // the device's address of h_patched
-    // device
-    unsigned char* d_in = nullptr;
-    int32_t* d_tokens = nullptr;
-    float* d_patched = nullptr;
-    std::vector<int> sid;
-    std::vector<unsigned char> stochastic;
-    std::vector<fsb::RowDesc> descs;   // descriptors in row order while a batch is staged (capacity kept between calls)
-    bool launched = false;
-    // Prepared batches: a redraw's copy reads h_in when its turn comes.  `ev_sent` is recorded behind it, but not for callers
-    // that were seen to wait for every step (it costs 3 us a step: 512 x 32768 sharded 72 -> 75).
-    bool sending = false;        // the copy may not have run yet
-    bool queues_steps = true;    // the caller does not wait for every step, as far as is known
-    bool redrawn = false;
-    cudaEvent_t ev_sent = nullptr;
-    const int32_t* hist_dev = nullptr;   // where the rows' penalty windows live: the batch's staged copy, or the engine's id pool
-
-    fsb::RowDesc* h_rows() const { return reinterpret_cast<fsb::RowDesc*>(h_in); }
-    int32_t* h_hist() const { return reinterpret_cast<int32_t*>(h_in + sizeof(fsb::RowDesc) * (size_t)cap_rows); }
-    fsb::RowDesc* d_rows() const { return reinterpret_cast<fsb::RowDesc*>(d_in); }
-    int32_t* d_hist() const { return reinterpret_cast<int32_t*>(d_in + sizeof(fsb::RowDesc) * (size_t)cap_rows); }
-    // the kernels' status word sits right behind the tokens, so that one copy brings both back
-    uint32_t* d_status() const { return reinterpret_cast<uint32_t*>(d_tokens + cap_rows); }
-    size_t in_bytes_used() const { return sizeof(fsb::RowDesc) * (size_t)cap_rows + sizeof(int32_t) * (size_t)(hist_ids + table_ints); }
-};
-
-struct fsb_handle {
-    int device = 0;
-    int max_rows = 0, max_vocab = 0;
-    int64_t max_hist = 0;
-    int sm_count = 0;
-    cudaStream_t stream = nullptr;
-    bool own_stream = false;
-    cudaStream_t side = nullptr;       // the full-vocabulary kernel of a mixed batch runs here, beside the streaming kernel
-    cudaEvent_t ev_fork = nullptr, ev_join = nullptr;
-    float softcap = 0.0f;
-    int32_t vocab_offset = 0;
-    int32_t global_vocab = 0;          // vocabulary sharding: columns of the whole row (0: this engine holds whole rows)
-    int launch_overlap = 0;
-    uint64_t call_no = 0;              // counts the calls that check their streams for duplicates
-    std::vector<Stream> streams;
-    std::vector<int> free_ids;
-    // device scratch shared by all batches of this handle
-    int32_t* d_kept_ids = nullptr;
-    double* d_kept_pr = nullptr;
-    int32_t* d_kept_n = nullptr;
-    bool kept_valid = false;
-    // prompt-lookup drafting: descriptors up, drafts stored into pinned memory by the kernel
-    fsb::LookupDesc* h_lookup = nullptr;
-    fsb::LookupDesc* d_lookup = nullptr;
-    int32_t* h_drafts = nullptr;
-    int32_t* h_drafts_dev = nullptr;   // the device's address of h_drafts
-    float* d_logits_stage = nullptr;   // device copy of host logits: max_rows x max_vocab, allocated with the engine
-    size_t logits_stage_elems = 0;
-    float* h_logits = nullptr;         // pinned memory through which a few host rows go to the device
-    int32_t* h_ids = nullptr;          // ring through which new history ids go to the device without waiting
-    size_t h_ids_pos = 0;
-    uint64_t* d_trace = nullptr;       // caller-owned diagnostics buffer, or null
-    fsb_batch* own = nullptr;          // the batch behind fsb_sample_batch / fsb_verify_windows
-    int32_t* d_pool = nullptr;         // resident histories: max_hist ids, carved into power-of-two regions
-    int64_t pool_top = 0;              // ids handed out so far (bump pointer)
-    std::vector<std::vector<int64_t>> pool_free;   // freed regions by size class
-    fsb_counters_t counters{};
-    std::string err;
-};
-
-namespace {
+namespace fsb {
 
 constexpr size_t kHostLogits = 256 * 1024;   // host logits that go through pinned memory of the engine's own (1 MB)
 constexpr size_t kIdRing = 64 * 1024;        // ids of the history ring
@@ -152,12 +44,6 @@ int fail(fsb_handle* h, int code, const char* fmt, ...) {
     return code;
 }
 
-#define FSB_CUDA(h, call)                                                                                  \
-    do {                                                                                                   \
-        cudaError_t e_ = (call);                                                                           \
-        if (e_ != cudaSuccess) return fail(h, FSB_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));      \
-    } while (0)
-
 bool is_greedy(const ferro_sampler_params& p) { return p.temperature <= 0.0f || p.top_k == 1; }   // src/sampler.cpp:19
 
 // Where a call's explicit histories lie: packed behind one another with offsets, or one array per stream (a scheduler
@@ -172,13 +58,14 @@ struct HistSource {
     const int32_t* data(int i) const { return off ? (flat ? flat + off[i] : nullptr) : lists[i]; }
 };
 
-// penalty window [b, len) of src/sampler.cpp:11-14; returns len when the window is empty or the penalty is off
-int64_t window_begin(const ferro_sampler_params& p, int64_t len) {
-    if (p.repetition_penalty == 1.0f || p.repeat_last_n == 0 || len <= 0) return len;
+int64_t window_start(const ferro_sampler_params& p, int64_t len) {
+    if (p.repeat_last_n == 0 || len <= 0) return len;
     int64_t b = (p.repeat_last_n > 0 && (int64_t)p.repeat_last_n < len) ? len - (int64_t)p.repeat_last_n : 0;
     if (p.penalty_from > 0) b = std::max<int64_t>(b, (int64_t)p.penalty_from);
     return std::min(b, len);
 }
+// penalty window [b, len); len when the window is empty or the repetition penalty is off
+int64_t window_begin(const ferro_sampler_params& p, int64_t len) { return p.repetition_penalty == 1.0f ? len : window_start(p, len); }
 
 void free_batch_buffers(fsb_batch* b) {
     if (!b) return;
@@ -450,11 +337,31 @@ int check_common(fsb_handle* h, int n_rows, int64_t ld, int n_vocab, const fsb_b
 }
 
 // ---- resident histories: regions of the engine's id pool, sizes 2^class ids (class >= 8) ----------------------
-void release_region(fsb_handle* h, Stream* s) {
-    if (s->pool_off >= 0) {
-        if ((size_t)s->pool_class >= h->pool_free.size()) h->pool_free.resize((size_t)s->pool_class + 1);
-        h->pool_free[(size_t)s->pool_class].push_back(s->pool_off);
+void give_region(fsb_handle* h, int64_t off, int cls) {
+    if (off < 0) return;
+    if ((size_t)cls >= h->pool_free.size()) h->pool_free.resize((size_t)cls + 1);
+    h->pool_free[(size_t)cls].push_back(off);
+}
+
+int take_region(fsb_handle* h, int64_t need, int64_t* off, int* cls) {
+    int c = 8;
+    while (((int64_t)1 << c) < need) ++c;
+    if ((size_t)c < h->pool_free.size() && !h->pool_free[(size_t)c].empty()) {
+        *off = h->pool_free[(size_t)c].back();
+        h->pool_free[(size_t)c].pop_back();
+    } else if (h->pool_top + ((int64_t)1 << c) <= h->max_hist) {
+        *off = h->pool_top;
+        h->pool_top += (int64_t)1 << c;
+    } else {
+        return fail(h, FSB_ERR_CAPACITY, "resident histories and biases need %lld more ids than the engine's pool of %lld holds", (long long)((int64_t)1 << c),
+                    (long long)h->max_hist);
     }
+    *cls = c;
+    return FSB_OK;
+}
+
+void release_region(fsb_handle* h, Stream* s) {
+    give_region(h, s->pool_off, s->pool_class);
     s->pool_off = -1;
     s->pool_class = -1;
     s->dev_len = 0;
@@ -463,19 +370,10 @@ void release_region(fsb_handle* h, Stream* s) {
 // Makes sure the stream's region holds at least `need` ids; moves what is already on the device if it must grow.
 int ensure_region(fsb_handle* h, Stream* s, int64_t need) {
     if (s->pool_off >= 0 && need <= ((int64_t)1 << s->pool_class)) return FSB_OK;
-    int c = 8;
-    while (((int64_t)1 << c) < need) ++c;
+    int c = -1;
     int64_t off = -1;
-    if ((size_t)c < h->pool_free.size() && !h->pool_free[(size_t)c].empty()) {
-        off = h->pool_free[(size_t)c].back();
-        h->pool_free[(size_t)c].pop_back();
-    } else if (h->pool_top + ((int64_t)1 << c) <= h->max_hist) {
-        off = h->pool_top;
-        h->pool_top += (int64_t)1 << c;
-    } else {
-        return fail(h, FSB_ERR_CAPACITY, "resident histories need %lld more ids than the engine's pool of %lld holds", (long long)((int64_t)1 << c),
-                    (long long)h->max_hist);
-    }
+    const int rc = take_region(h, need, &off, &c);
+    if (rc) return rc;
     if (s->pool_off >= 0 && s->dev_len > 0)
         FSB_CUDA(h, cudaMemcpyAsync(h->d_pool + off, h->d_pool + s->pool_off, sizeof(int32_t) * (size_t)s->dev_len, cudaMemcpyDeviceToDevice, h->stream));
     const int64_t kept = s->dev_len;
@@ -486,14 +384,8 @@ int ensure_region(fsb_handle* h, Stream* s, int64_t need) {
     return FSB_OK;
 }
 
-// Brings the device copy of the stream's history up to date with its host mirror.
-int sync_history(fsb_handle* h, Stream* s) {
-    const int64_t n = (int64_t)s->hist.size();
-    if (n <= s->dev_len) return FSB_OK;
-    const int rc = ensure_region(h, s, n);
-    if (rc) return rc;
-    const size_t count = (size_t)(n - s->dev_len);
-    const int32_t* src = s->hist.data() + s->dev_len;
+int upload_ids(fsb_handle* h, int64_t pool_off, const int32_t* ids, size_t count) {
+    const int32_t* src = ids;
     if (count <= kIdRing) {   // through the pinned ring: nothing to wait for until it comes round again
         if (h->h_ids_pos + count > kIdRing) {
             FSB_CUDA(h, cudaStreamSynchronize(h->stream));
@@ -502,8 +394,18 @@ int sync_history(fsb_handle* h, Stream* s) {
         src = static_cast<const int32_t*>(std::memcpy(h->h_ids + h->h_ids_pos, src, sizeof(int32_t) * count));
         h->h_ids_pos += count;
     }
-    FSB_CUDA(h, cudaMemcpyAsync(h->d_pool + s->pool_off + s->dev_len, src, sizeof(int32_t) * count, cudaMemcpyHostToDevice, h->stream));
+    FSB_CUDA(h, cudaMemcpyAsync(h->d_pool + pool_off, src, sizeof(int32_t) * count, cudaMemcpyHostToDevice, h->stream));
     if (count > kIdRing) FSB_CUDA(h, cudaStreamSynchronize(h->stream));   // the source is pageable host memory that may change after return
+    return FSB_OK;
+}
+
+// Brings the device copy of the stream's history up to date with its host mirror.
+int sync_history(fsb_handle* h, Stream* s) {
+    const int64_t n = (int64_t)s->hist.size();
+    if (n <= s->dev_len) return FSB_OK;
+    int rc = ensure_region(h, s, n);
+    if (rc == FSB_OK) rc = upload_ids(h, s->pool_off + s->dev_len, s->hist.data() + s->dev_len, (size_t)(n - s->dev_len));
+    if (rc) return rc;
     s->dev_len = n;
     return FSB_OK;
 }
@@ -632,7 +534,7 @@ int scatter_patched(fsb_handle* h, const fsb_batch* b, float* logits_host, const
 // The common tail of the synchronous calls: upload, (stage host logits), launch, fetch, (write back to host).
 // `window_append` > 0: a resident verification call of that many streams whose accepted tokens are stored behind the
 // histories (see verify_windows_impl).
-int run_staged(fsb_handle* h, fsb_batch* b, const float* logits, unsigned flags, int32_t* tokens_out, int window_append = 0) {
+int run_staged(fsb_handle* h, fsb_batch* b, const float* logits, unsigned flags, int32_t* tokens_out, int window_append) {
     const bool on_host = (flags & FSB_LOGITS_ON_HOST) != 0;
     const bool host_wb = on_host && (flags & FSB_WRITE_BACK) && b->gather_ids > 0;
     // the streaming kernel hands the penalised values over itself; rows of the full-vocabulary kernel have theirs gathered
@@ -659,7 +561,15 @@ int run_staged(fsb_handle* h, fsb_batch* b, const float* logits, unsigned flags,
     return rc;
 }
 
-}  // namespace
+void release_head(fsb_head* head) {
+    if (head->d_weights) cudaFree(head->d_weights);
+    if (head->d_scales) cudaFree(head->d_scales);
+    delete head;
+}
+
+}  // namespace fsb
+
+using namespace fsb;
 
 // ================================================================================================ C ABI
 extern "C" {
@@ -740,6 +650,12 @@ int fsb_create(int device, int max_rows, int max_vocab, int64_t max_hist_ids, fs
         cudaMallocHost(reinterpret_cast<void**>(&h->h_drafts), sizeof(int32_t) * (size_t)max_rows * fsb::kDraftStride) != cudaSuccess ||
         cudaHostGetDevicePointer(reinterpret_cast<void**>(&h->h_drafts_dev), h->h_drafts, 0) != cudaSuccess)
         return bail(FSB_ERR_CUDA);
+    // adjusted steps
+    if (cudaMalloc(reinterpret_cast<void**>(&h->d_row_state), sizeof(uint32_t) * (size_t)max_rows) != cudaSuccess ||
+        cudaMemset(h->d_row_state, 0, sizeof(uint32_t) * (size_t)max_rows) != cudaSuccess ||
+        cudaMallocHost(reinterpret_cast<void**>(&h->h_empty), sizeof(uint32_t)) != cudaSuccess ||
+        cudaHostGetDevicePointer(reinterpret_cast<void**>(&h->h_empty_dev), h->h_empty, 0) != cudaSuccess)
+        return bail(FSB_ERR_CUDA);
     if (alloc_batch(h, max_rows, max_hist_ids, std::max<int64_t>(max_hist_ids, 1), &h->own) != FSB_OK) return bail(FSB_ERR_CUDA);
     *out = h;
     return FSB_OK;
@@ -753,6 +669,12 @@ int fsb_destroy(fsb_handle* h) {
         free_batch_buffers(h->own);
         delete h->own;
     }
+    while (!h->heads.empty()) {
+        release_head(h->heads.back());
+        h->heads.pop_back();
+    }
+    if (h->d_row_state) cudaFree(h->d_row_state);
+    if (h->h_empty) cudaFreeHost(h->h_empty);
     if (h->d_kept_ids) cudaFree(h->d_kept_ids);
     if (h->d_kept_pr) cudaFree(h->d_kept_pr);
     if (h->d_kept_n) cudaFree(h->d_kept_n);
@@ -835,6 +757,8 @@ int fsb_stream_open(fsb_handle* h, const ferro_sampler_params* p, int* stream_id
     s.seed_used = p->seed ? p->seed : (uint64_t)std::random_device{}();   // src/sampler.h:25
     s.rng.seed(s.seed_used);
     s.draws = 0;
+    s.frequency = s.presence = 0.0f;
+    s.n_bias = 0;
     s.open = true;
     *stream_id = id;
     return FSB_OK;
@@ -845,6 +769,9 @@ int fsb_stream_close(fsb_handle* h, int stream_id) {
     Stream* s = get_stream(h, stream_id);
     if (!s) return fail(h, FSB_ERR_STREAM_ID, "unknown stream id %d", stream_id);
     release_region(h, s);
+    give_region(h, s->bias_off, s->bias_class);
+    s->bias_off = -1;
+    s->n_bias = 0;
     s->hist.clear();
     s->hist.shrink_to_fit();
     s->open = false;

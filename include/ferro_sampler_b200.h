@@ -54,7 +54,8 @@ typedef enum fsb_status {
     FSB_ERR_CUDA = -4,      /* a CUDA runtime call failed; text in fsb_last_error */
     FSB_ERR_STREAM_ID = -5, /* unknown or closed stream id */
     FSB_ERR_NO_DEVICE = -6, /* no usable CUDA device */
-    FSB_ERR_DEVICE = -7     /* a kernel reported an internal error through its status word */
+    FSB_ERR_DEVICE = -7,    /* a kernel reported an internal error through its status word */
+    FSB_ERR_EMPTY = -8      /* masks and biases leave a row no token (fsb_sample_batch_adjusted, fsb_sample_hidden) */
 } fsb_status;
 
 /* flags of fsb_sample_batch / fsb_verify_windows / fsb_batch_prepare */
@@ -282,6 +283,76 @@ FSB_API int fsb_batch_check(fsb_handle* h, fsb_batch* b);
 /* Number of kernels one fsb_batch_launch enqueues (for launch accounting). */
 FSB_API int fsb_batch_kernel_count(const fsb_batch* b);
 FSB_API int fsb_batch_free(fsb_handle* h, fsb_batch* b);
+
+/* ---- in front of the sampler: logit adjustment, LM head ------------------------------------------------------ */
+
+/* Element types of logits, hidden states and scales. */
+enum { FSB_F32 = 0, FSB_BF16 = 1, FSB_F16 = 2 };
+
+/* What a request asks of its logits beside the sampler's parameters; both belong to the stream and end with it.
+ *   fsb_stream_penalties_set   frequency and presence penalty (finite; 0 = off, the value after fsb_stream_open);
+ *   fsb_stream_bias_set        replaces the stream's logit biases: n token ids, each at most once, and what is added to
+ *                              their logits (finite, or minus infinity: never this token).  n = 0 removes them.  The list
+ *                              lives in the id pool of the resident histories and takes 2n ids there (regions of
+ *                              power-of-two size, at least 256).  FSB_ERR_CAPACITY when the pool cannot hold it; the old
+ *                              biases then stay.
+ * fsb_adjust_logits and the calls built on it apply them; the plain sampling calls do not look at them.
+ * No reference counterpart. */
+FSB_API int fsb_stream_penalties_set(fsb_handle* h, int stream_id, float frequency, float presence);
+FSB_API int fsb_stream_bias_set(fsb_handle* h, int stream_id, const int32_t* ids, const float* values, int n);
+
+/* Row i of `logits` ([n_rows][ld] of logits_type, device memory) as stream stream_ids[i] wants it sampled, into row i of
+ * `out` ([n_rows][out_ld]; fp32, or the type of the logits).  With c(v) the number of times token v stands in the stream's
+ * penalty window - its resident history (fsb_stream_history_*) cut by repeat_last_n and penalty_from, as for the repetition
+ * penalty, src/sampler.cpp:11-14 -, for every column in this order, in fp32 and rounded once at the end:
+ *     x = cap * tanhf(x / cap)                    if the engine has a softcap (fsb_set_softcap)
+ *     x = x > 0 ? x / repetition : x * repetition     if c(v) > 0                                (src/sampler.cpp:17)
+ *     x = x - (frequency * c(v) + presence)       if c(v) > 0
+ *     x = x + bias(v)
+ *     x = -infinity                               if the row has a mask, and it does not allow v
+ * What lies in a masked column of `logits` (NaN, say) does not matter.  A mask that allows nothing leaves a row of minus
+ * infinities.  masks: [n_masks][mask_ld] 32-bit words in device memory, bit v % 32 of word v / 32 allows token v
+ * (mask_ld >= the words of the whole vocabulary; with a vocabulary shard v = column + offset); mask_rows[i] (host memory)
+ * is the mask of row i, or -1 for a row without one.  mask_rows = NULL: row i has mask i.  masks = NULL: no row has one.
+ * `out` may be `logits` with the same type and stride (in place), and must not overlap it otherwise.  A stream may stand for
+ * several rows.  Columns from n_vocab on are neither read nor written.
+ * Asynchronous on the engine's stream; stream_ids and mask_rows are read before the call returns.  Not inside a stream
+ * capture (FSB_ERR_INVALID): a replay would see the histories of the capture.  No reference counterpart. */
+FSB_API int fsb_adjust_logits(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab,
+                              const uint32_t* masks, int64_t mask_ld, int n_masks, const int32_t* mask_rows, void* out, int out_type, int64_t out_ld);
+
+/* fsb_sample_batch_resident over adjusted logits: the rows of fsb_adjust_logits, sampled.  The adjusted rows are kept by the
+ * engine, the caller's stay as they are; the repetition penalty and the softcap are applied once, by the adjustment.
+ * `flags`: FSB_APPEND_SAMPLED, FSB_KEEP_KEPT_SET.  A stream may appear once per call.  FSB_ERR_EMPTY if a row has nothing left
+ * above minus infinity: no token is returned, nothing is appended, and no engine has advanced. */
+FSB_API int fsb_sample_batch_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab,
+                                      const uint32_t* masks, int64_t mask_ld, int n_masks, const int32_t* mask_rows, int32_t* tokens_out, unsigned flags);
+
+/* An LM head with 4-bit weights and a scale per group: logit v of hidden state x is
+ *     sum over the groups g of scale[v][g] * sum over k in g of (q[v][k] - 8) * x[k].
+ * weights [n_vocab][n_hidden / 2] bytes, two weights to a byte, the first in the low four bits; scales [n_vocab]
+ * [n_hidden / group], FSB_F16 or FSB_BF16; group 32, 64 or 128, a divisor of n_hidden (at most FSB_MAX_HIDDEN).  Both in
+ * device memory, or with FSB_WEIGHTS_ON_HOST in host memory.  fsb_head_create copies them into the layout that the kernels
+ * read and waits for that; the caller's arrays are not needed afterwards.  It allocates device memory: n_hidden / 2 bytes a
+ * row and the scales, rows rounded up to 128.  A head belongs to the engine that created it and is freed with it at the
+ * latest.  (The dequantisation of a Q4_0 block: 32 weights, d * (q - 8).)  No reference counterpart in this form: the
+ * reference's heads are Q8 (q8gemv). */
+typedef struct fsb_head fsb_head;
+#define FSB_WEIGHTS_ON_HOST 1u
+#define FSB_MAX_HIDDEN 16384
+FSB_API int fsb_head_create(fsb_handle* h, int n_vocab, int n_hidden, int group, const uint8_t* weights, const void* scales, int scale_type,
+                            unsigned flags, fsb_head** out);
+FSB_API int fsb_head_free(fsb_handle* h, fsb_head* head);
+/* logits [n_rows][ld] fp32 of the hidden states [n_rows][ld_hidden] (FSB_BF16 or FSB_F16), both in device memory, which must
+ * not overlap.  Products are exact, sums and scales fp32.  Asynchronous on the engine's stream, without any workspace: may be
+ * captured into a CUDA graph.  At most 65535 rows, however many the engine was created for. */
+FSB_API int fsb_head_logits(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidden, int hidden_type, int64_t ld_hidden, float* logits,
+                            int64_t ld);
+/* A decode step from hidden states to tokens: fsb_head_logits into the engine's own memory, then what
+ * fsb_sample_batch_adjusted does with those logits (flags and errors as there; the head's vocabulary must fit the engine). */
+FSB_API int fsb_sample_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const int* stream_ids, const void* hidden, int hidden_type,
+                              int64_t ld_hidden, const uint32_t* masks, int64_t mask_ld, int n_masks, const int32_t* mask_rows, int32_t* tokens_out,
+                              unsigned flags);
 
 /* ---- counters --------------------------------------------------------------------------------------------- */
 typedef struct fsb_counters_t {
