@@ -195,19 +195,26 @@ def _logits_pointer(logits, n_vocab, flags):
     raise TypeError("logits: numpy array or device tensor expected")
 
 
+_kinds: dict = {}   # element types by tensor dtype, as they come up
+
+
 def _device_rows(t, device: int, what: str):
     """A two-dimensional device tensor (rows contiguous): its address, element type and row stride."""
-    kind = ELEMENT_TYPES.get(str(t.dtype).rsplit(".", 1)[-1])
+    dtype = t.dtype
+    kind = _kinds.get(dtype)
     if kind is None:
-        raise TypeError(f"{what}: {t.dtype} is not one of {', '.join(ELEMENT_TYPES)}")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        kind = _kinds[dtype] = ELEMENT_TYPES.get(str(dtype).rsplit(".", 1)[-1], -1)
+    if kind < 0:
+        raise TypeError(f"{what}: {dtype} is not one of {', '.join(ELEMENT_TYPES)}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError(f"{what}: a matrix with contiguous rows is expected")
     _check_device(t, device, what)
-    return int(t.data_ptr()), kind, int(t.stride(0)) if t.shape[0] > 1 else max(int(t.stride(0)), int(t.shape[1]))
+    return t.data_ptr(), kind, stride[0] if shape[0] > 1 else max(stride[0], shape[1])
 
 
 def _check_device(t, device: int, what: str):
-    if t.device.type != "cuda" or t.device.index != device:
+    if not t.is_cuda or t.get_device() != device:
         raise ValueError(f"{what} is on {t.device}, the engine on cuda:{device}")
 
 
@@ -220,11 +227,11 @@ def _mask_words(masks, device: int):
     if masks.dim() != 2 or (masks.shape[1] > 1 and masks.stride(1) != 1):
         raise ValueError("masks: a matrix of words with contiguous rows is expected")
     _check_device(masks, device, "masks")
-    # (one row alone may have any stride: what lies in it is what counts)
-    ld = int(masks.shape[1]) if masks.shape[0] <= 1 else int(masks.stride(0))
-    if ld < masks.shape[1]:
+    n, words = masks.shape
+    ld = words if n <= 1 else masks.stride(0)   # (one row alone may have any stride: what lies in it is what counts)
+    if ld < words:
         raise ValueError("masks: rows overlap")
-    return int(masks.data_ptr()), ld, int(masks.shape[0])
+    return masks.data_ptr(), ld, n
 
 
 class Batch:

@@ -5,10 +5,10 @@
 //     x = cap * tanhf(x / cap);  c(v) > 0: x = (x > 0 ? x / p : x * p) - (f * c(v) + q);  x += bias(v);  masked: x = -inf
 // in fp32, rounded once when it is stored.
 //
-// One pass over the logits, bound by its bytes.  A CTA takes kTile columns of one row.  Its mask bits come first, and vectors
-// of logits that are masked altogether are not read (a grammar leaves a handful of tokens as often as not).  Few columns stand
-// in the window or have a bias: they are marked in a bitmap, and only marked columns look at the counts (in shared memory,
-// cleared where they are marked and nowhere else) and the bias list.
+// One pass over the logits, bound by its bytes.  A CTA takes a tile of one row, batch by batch of 16 columns a thread.  A batch's
+// mask bits are fetched two batches ahead and its logits one ahead; vectors of logits that are masked altogether are not read (a
+// grammar leaves a handful of tokens as often as not).  While the first batch is on its way the window is scanned once: occurrences
+// in the tile are counted in shared memory, and bitmaps mark the few columns that have to look at their count or their bias.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -21,148 +21,278 @@ namespace fsb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 4096;                     // columns of a CTA
-constexpr int kCols = kTile / kThreads;         // ... and of a thread
+constexpr int kCols = 16;                       // columns of a thread in a batch
+constexpr int kBatch = kThreads * kCols;
+constexpr int kBatchesMax = 4;                  // batches of a tile
 constexpr int kBlockRows = 512;                 // rows whose descriptors go with one launch
 
 template <int ROWS>
 struct Params {
     AdjustArgs a;
+    int32_t tile;      // columns of a CTA
     AdjustRow rows[ROWS];
 };
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <class T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-
-// N elements that are loaded and stored together, 16 bytes at a time.
-template <class T, int N>
-struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
-    T v[N];
+// VEC elements as 32-bit words (a lone 16-bit element in the lower half of one), loaded and stored in as few pieces as there are.
+template <class T, int VEC>
+struct Raw {
+    static constexpr int kWords = VEC * (int)sizeof(T) < 4 ? 1 : VEC * (int)sizeof(T) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kWords == 8) {
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p));
+        } else if constexpr (kWords == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (kWords == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x, w[1] = v.y;
+        } else if constexpr (sizeof(T) == 2) {
+            w[0] = *reinterpret_cast<const unsigned short*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kWords == 8)   // (a whole sector: two stores of 16 bytes would each write half of one)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                         "r"(w[6]), "r"(w[7])
+                         : "memory");
+        else if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else if constexpr (sizeof(T) == 2) *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+        else *reinterpret_cast<uint32_t*>(p) = w[0];
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1])));
+    }
+    __device__ __forceinline__ void set(const float (&v)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i < VEC ? 2 * i : 0], v[2 * i + 1 < VEC ? 2 * i + 1 : 0]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(v[2 * i < VEC ? 2 * i : 0], v[2 * i + 1 < VEC ? 2 * i + 1 : 0]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+    }
 };
 
-// The mask bits of the N <= 16 columns whose first token id is `id`.  A word is read where one of the columns [id, id + n) lies in it.
-__device__ __forceinline__ unsigned mask_bits(const uint32_t* mask, int id, int n) {
-    const int w = id >> 5, shift = id & 31;
-    const unsigned lo = __ldg(mask + w);
-    const unsigned hi = shift + n > 32 ? __ldg(mask + w + 1) : 0u;
-    return __funnelshift_r(lo, hi, shift);
+// cap * tanh(v / cap), inv = 1 / cap.  The division: a product and one correction by its exact remainder.  tanh a = 1 - 2 / (e^2a + 1), and
+// the first terms of its Taylor series where that would cancel (below 0.35 the next one is less than 2^-26 of the sum): within 2^-21
+// relative, as good as tanhf in half the instructions, of which a row of soft-capped fp32 logits is made (64 x 262144: 43 -> 40 us, 33 with eight columns a vector).
+__device__ __forceinline__ float capped(float v, float cap, float inv) {
+    // from ten caps on tanh is 1 in fp32 (and infinity would have no remainder); NaN stays
+    float x;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(v), "f"(10.0f * cap));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-10.0f * cap));
+    const float q = __fmul_rn(x, inv), u = __fmaf_rn(__fmaf_rn(-q, cap, x), inv, q);
+    const float s = __fmul_rn(u, u);
+    float p = __fmaf_rn(s, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    p = __fmaf_rn(s, p, -17.0f / 315.0f);
+    p = __fmaf_rn(s, p, 2.0f / 15.0f);
+    p = __fmaf_rn(s, p, -1.0f / 3.0f);
+    const float small = __fmaf_rn(__fmul_rn(s, p), u, u);
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(u) * 2.8853900817779268f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    const float big = copysignf(__fmaf_rn(-2.0f, r, 1.0f), u);
+    return __fmul_rn(cap, fabsf(u) < 0.35f ? small : big);
 }
 
-template <class TI, class TO, int VEC, int ROWS>
-__global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant__ Params<ROWS> P) {
+// Shared memory of a tile: occurrences (16 bits a column where the window is shorter than 65536 ids, else 32); for every 32
+// columns the bitmaps of those that occur and of those with a bias, and the place of the first bias in the row's list.
+template <bool WIDE>
+struct Special {
+    unsigned* count;
+    uint2* marks;      // occurs, biased
+    int* bias_at;
+    static __host__ __device__ constexpr int bytes(int tile) { return tile * (WIDE ? 4 : 2) + 3 * (tile / 8); }
+    __device__ __forceinline__ Special(unsigned char* smem, int tile) {
+        count = reinterpret_cast<unsigned*>(smem);
+        marks = reinterpret_cast<uint2*>(smem + tile * (WIDE ? 4 : 2));
+        bias_at = reinterpret_cast<int*>(marks + tile / 32);
+    }
+    __device__ __forceinline__ void add(unsigned c) const {
+        if (WIDE) atomicAdd(&count[c], 1u);
+        else atomicAdd(&count[c >> 1], 1u << ((c & 1) * 16));
+        atomicOr(&marks[c >> 5].x, 1u << (c & 31));   // (asking first, or the count's old value, is slower: 14.4 -> 16.6, 17.2 us for 16 windows of 16384 ids)
+    }
+    __device__ __forceinline__ float times(int c) const { return (float)(WIDE ? count[c] : count[c >> 1] >> ((c & 1) * 16) & 0xffffu); }
+};
+
+template <class TI, class TO, int VEC, int ROWS, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 4) adjust_kernel(const __grid_constant__ Params<ROWS> P) {
     constexpr int kVecs = kCols / VEC;
-    __shared__ unsigned marked[kTile / 32];
-    __shared__ int count[kTile];
+    constexpr unsigned kAll = (1u << VEC) - 1u, kEvery = (1u << kCols) - 1u;
+    extern __shared__ __align__(16) unsigned char smem[];
     const AdjustArgs& a = P.a;
     const int row = (int)blockIdx.y, tid = (int)threadIdx.x;
     const AdjustRow& R = P.rows[row];
-    const int c0 = (int)blockIdx.x * kTile, n = min(kTile, a.n_vocab - c0);   // this CTA's columns
-    const int id0 = c0 + a.vocab_offset;                                      // token id of its first one
-    const TI* in = static_cast<const TI*>(a.in) + (int64_t)row * a.ld + c0;
-    TO* out = static_cast<TO*>(a.out) + (int64_t)row * a.out_ld + c0;
+    const int tile = P.tile, c0 = (int)blockIdx.x * tile, n = min(tile, a.n_vocab - c0);   // this CTA's columns
+    const int batches = (n + kBatch - 1) / kBatch;
+    const int id0 = c0 + a.vocab_offset;                                                   // token id of its first one
+    const int own = tid * VEC;                                                             // the thread's first column in a row of vectors
+    const TI* in = static_cast<const TI*>(a.in) + (int64_t)row * a.ld + c0 + own;
+    TO* out = static_cast<TO*>(a.out) + (int64_t)row * a.out_ld + c0 + own;
+    const uint32_t* mask = R.mask_row >= 0 ? a.masks + (int64_t)R.mask_row * a.mask_ld + ((id0 + own) >> 5) : nullptr;
+    const int shift = (id0 + own) & 31;
+    const Special<WIDE> S(smem, tile);
 
-    // mask bits, then the logits that they leave
-    unsigned keep[kVecs];
+    // A batch's columns that are there and allowed, VEC bits for each of the thread's vectors.  A word of the mask is read only if
+    // one of the columns lies in it.
+    auto allowed = [&](int b) {
+        unsigned keep = 0u;
+        const int there = n - b * kBatch - own;   // columns from the thread's first one on
+        if ((kVecs - 1) * kThreads * VEC + VEC <= there) keep = kEvery;
+        else {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int c = (i * kThreads + tid) * VEC;
-        const int m = min(VEC, n - c);
-        keep[i] = m <= 0 ? 0u : (1u << m) - 1u;
-        if (R.mask_row >= 0 && m > 0) keep[i] &= mask_bits(a.masks + (int64_t)R.mask_row * a.mask_ld, id0 + c, m);
-    }
-    Pack<TI, VEC> x[kVecs];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int c = (i * kThreads + tid) * VEC;
-        if (keep[i] == 0u) continue;
-        if (c + VEC <= n) {
-            x[i] = *reinterpret_cast<const Pack<TI, VEC>*>(in + c);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (c + j < n) x[i].v[j] = in[c + j];
+            for (int i = 0; i < kVecs; ++i) keep |= ((1u << max(0, min(VEC, there - i * kThreads * VEC))) - 1u) << (i * VEC);
         }
-    }
-
-    const bool special = R.hist_len > 0 || R.n_bias > 0;
-    const int32_t* hist = a.pool + R.hist_begin;
-    const int32_t* bias_ids = a.pool + R.bias_begin;
-    if (special) {
-        if (tid < kTile / 32) marked[tid] = 0u;
-        __syncthreads();
-        for (int i = tid; i < R.hist_len; i += kThreads) {
-            const unsigned c = (unsigned)__ldg(hist + i) - (unsigned)id0;
-            if (c < (unsigned)n) {
-                atomicOr(&marked[c >> 5], 1u << (c & 31));
-                count[c] = 0;
+        if (mask) {
+            const uint32_t* p = mask + b * (kBatch / 32);
+            unsigned bits = 0u;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int m = min(VEC, there - i * kThreads * VEC);
+                if (m <= 0) continue;
+                unsigned word = __ldg(p + i * (kThreads * VEC / 32)) >> shift;
+                if (VEC > 1 && shift + m > 32) word |= __ldg(p + i * (kThreads * VEC / 32) + 1) << (32 - shift);
+                bits |= (word & kAll) << (i * VEC);
+            }
+            keep &= bits;
+        }
+        return keep;
+    };
+    Raw<TI, VEC> x[kVecs];
+    auto fetch = [&](int b, int i) {
+        const int c = b * kBatch + i * kThreads * VEC;
+        if (own + c + VEC <= n) x[i].load(in + c);
+        else {   // the row's last vector
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                Raw<TI, 1> e;
+                e.w[0] = 0u;
+                if (own + c + j < n) e.load(in + c + j);
+                if constexpr (sizeof(TI) == 4) x[i].w[j] = e.w[0];
+                else x[i].w[j >> 1] = j & 1 ? x[i].w[j >> 1] | e.w[0] << 16 : e.w[0];
             }
         }
-        for (int i = tid; i < R.n_bias; i += kThreads) {
+    };
+
+    // the first batch's logits (masked or not), its mask bits and the window's first ids are fetched together
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+        if (own + i * kThreads * VEC < n) fetch(0, i);
+    unsigned keep = allowed(0);
+    // four ids at a time, from the 16-byte boundary before the window on (regions of the id pool start and end on such)
+    const int lead = (int)(R.hist_begin & 3), quads = R.hist_len > 0 ? (lead + R.hist_len + 3) >> 2 : 0;
+    const int4* ids = reinterpret_cast<const int4*>(a.pool + R.hist_begin - lead);
+    const int32_t* bias_ids = a.pool + R.bias_begin;
+    int4 quad = make_int4(0, 0, 0, 0);
+    if (tid < quads) quad = __ldg(ids + tid);
+    const bool special = R.hist_len > 0 || R.n_bias > 0;
+    if (special) {
+        for (int i = tid; i < Special<WIDE>::bytes(tile) / 16; i += kThreads) reinterpret_cast<int4*>(smem)[i] = make_int4(0, 0, 0, 0);
+    }
+    unsigned next = batches > 1 ? allowed(1) : 0u;
+    if (special) {
+        __syncthreads();
+        for (int q = tid; q < quads; q += kThreads) {
+            const int4 v = quad;
+            if (q + kThreads < quads) quad = __ldg(ids + q + kThreads);
+            const int at = q * 4 - lead, id[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned c = (unsigned)id[j] - (unsigned)id0;
+                if (c < (unsigned)n && (unsigned)(at + j) < (unsigned)R.hist_len) S.add(c);
+            }
+        }
+        for (int i = tid; i < R.n_bias; i += kThreads) {   // (no id stands there twice, and they ascend)
             const unsigned c = (unsigned)__ldg(bias_ids + i) - (unsigned)id0;
             if (c < (unsigned)n) {
-                atomicOr(&marked[c >> 5], 1u << (c & 31));
-                count[c] = 0;
+                atomicMax(&S.bias_at[c >> 5], R.n_bias - i);
+                atomicOr(&S.marks[c >> 5].y, 1u << (c & 31));
             }
-        }
-        __syncthreads();
-        for (int i = tid; i < R.hist_len; i += kThreads) {
-            const unsigned c = (unsigned)__ldg(hist + i) - (unsigned)id0;
-            if (c < (unsigned)n) atomicAdd(&count[c], 1);
         }
         __syncthreads();
     }
 
-    const float none = -__int_as_float(0x7f800000);
+    const float none = -__int_as_float(0x7f800000), inv = __frcp_rn(a.softcap);
     bool any = false;
+    for (int b = 0; b < batches; ++b) {
+        const unsigned now = keep;
+        keep = next;
+        next = b + 2 < batches ? allowed(b + 2) : 0u;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int c = (i * kThreads + tid) * VEC;
-        Pack<TO, VEC> y;
-        unsigned mark = 0u;
-        if (special && keep[i] != 0u) mark = (marked[c >> 5] >> (c & 31)) & ((1u << VEC) - 1u);
+        for (int i = 0; i < kVecs; ++i) {
+            const int c = b * kBatch + i * kThreads * VEC;   // the thread's vector starts at column c + own
+            const unsigned k = now >> (i * VEC) & kAll;
+            float v[VEC];
+            if (k) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            float v = none;
-            if (keep[i] >> j & 1u) {
-                v = to_f32(x[i].v[j]);
-                if (a.softcap > 0.0f) v = __fmul_rn(a.softcap, tanhf(__fdiv_rn(v, a.softcap)));
-                if (mark >> j & 1u) {
-                    const int k = count[c + j];
-                    if (k > 0) {
-                        v = v > 0.0f ? __fdiv_rn(v, R.repetition) : __fmul_rn(v, R.repetition);
-                        v -= __fmaf_rn(R.frequency, (float)k, R.presence);
-                    }
-                    // its place in the bias list, if it has one: ids ascend
-                    int lo = 0, hi = R.n_bias;
-                    while (lo < hi) {
-                        const int mid = (lo + hi) >> 1;
-                        if (__ldg(bias_ids + mid) < id0 + c + j) lo = mid + 1;
-                        else hi = mid;
-                    }
-                    if (lo < R.n_bias && __ldg(bias_ids + lo) == id0 + c + j) {
-                        const float b = __int_as_float(__ldg(bias_ids + R.n_bias + lo));
-                        v = b == none ? none : v + b;
+                for (int j = 0; j < VEC; ++j) v[j] = x[i].get(j);
+            }
+            if (keep >> (i * VEC) & kAll) fetch(b + 1, i);
+            if (k == 0u) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = none;
+            } else {
+                if (a.softcap > 0.0f) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[j] = capped(v[j], a.softcap, inv);
+                }
+                if (special) {
+                    const int at = c / 32 + own / 32, bit = own & 31;
+                    const uint2 mark = S.marks[at];
+                    for (unsigned m = (mark.x | mark.y) >> bit & k; m; m &= m - 1u) {   // few: a loop keeps the code short
+                        const int j = __ffs(m) - 1;
+                        float y = v[0];
+#pragma unroll
+                        for (int q = 1; q < VEC; ++q) y = j == q ? v[q] : y;
+                        if (mark.x >> (bit + j) & 1u) {
+                            y = y > 0.0f ? __fdiv_rn(y, R.repetition) : __fmul_rn(y, R.repetition);
+                            y -= __fmaf_rn(R.frequency, S.times(c + own + j), R.presence);
+                        }
+                        if (mark.y >> (bit + j) & 1u) {
+                            const int place = R.n_bias - S.bias_at[at] + __popc(mark.y & ((1u << (bit + j)) - 1u));
+                            const float f = __int_as_float(__ldg(bias_ids + R.n_bias + place));
+                            y = f == none ? none : y + f;
+                        }
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q) v[q] = j == q ? y : v[q];
                     }
                 }
-            }
-            any = any || v > none;
-            y.v[j] = from_f32<TO>(v);
-        }
-        if (c + VEC <= n) {
-            *reinterpret_cast<Pack<TO, VEC>*>(out + c) = y;
-        } else {
+                if (k != kAll) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (c + j < n) out[c + j] = y.v[j];
+                    for (int j = 0; j < VEC; ++j)
+                        if (!(k >> j & 1u)) v[j] = none;
+                }
+                if (a.row_state) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) any = any || v[j] > none;
+                }
+            }
+            if (c + own + VEC <= n) {
+                Raw<TO, VEC> y;
+                y.set(v);
+                y.store(out + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float one[1] = {v[j]};
+                    Raw<TO, 1> y;
+                    y.set(one);
+                    if (c + own + j < n) y.store(out + c + j);
+                }
+            }
         }
     }
 
@@ -184,13 +314,22 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant_
     }
 }
 
-template <class TI, class TO, int VEC, int ROWS>
+template <class TI, class TO, int VEC, int ROWS, bool WIDE>
 int launch_rows(const AdjustArgs& a, const AdjustRow* rows, int n_rows, cudaStream_t stream) {
     Params<ROWS> p;
     p.a = a;
     std::copy(rows, rows + n_rows, p.rows);
-    const dim3 grid((unsigned)((a.n_vocab + kTile - 1) / kTile), (unsigned)n_rows);
-    adjust_kernel<TI, TO, VEC, ROWS><<<grid, kThreads, 0, stream>>>(p);
+    // Long tiles share one scan of the window and keep the loads going; short ones keep every SM busy where there is little to do.
+    const int row_batches = (a.n_vocab + kBatch - 1) / kBatch, most = std::min(WIDE ? 2 : kBatchesMax, row_batches);
+    int batches = 1;
+    int64_t best = 0;
+    for (int b = 1; b <= most; ++b) {
+        const int64_t ctas = (int64_t)((row_batches + b - 1) / b) * n_rows, waves = (ctas + 4 * 148 - 1) / (4 * 148), cost = waves * (10 * b + 7);
+        if (best == 0 || cost < best) best = cost, batches = b;
+    }
+    p.tile = batches * kBatch;
+    const dim3 grid((unsigned)((a.n_vocab + p.tile - 1) / p.tile), (unsigned)n_rows);
+    adjust_kernel<TI, TO, VEC, ROWS, WIDE><<<grid, kThreads, (size_t)Special<WIDE>::bytes(p.tile), stream>>>(p);
     return (int)cudaGetLastError();
 }
 
@@ -203,24 +342,30 @@ int launch_vec(const AdjustArgs& a, const AdjustRow* rows, cudaStream_t stream, 
         b.out = static_cast<TO*>(a.out) + (int64_t)at * a.out_ld;
         b.first_row = at;
         b.row_state = a.row_state ? a.row_state + at : nullptr;
-        int e;
-        if (n <= 16) e = launch_rows<TI, TO, VEC, 16>(b, rows + at, n, stream);
-        else if (n <= 96) e = launch_rows<TI, TO, VEC, 96>(b, rows + at, n, stream);
-        else e = launch_rows<TI, TO, VEC, kBlockRows>(b, rows + at, n, stream);
+        int longest = 0, e;
+        for (int i = 0; i < n; ++i) longest = std::max(longest, rows[at + i].hist_len);
+        if (longest >= 65536) e = launch_rows<TI, TO, VEC, kBlockRows, true>(b, rows + at, n, stream);
+        else if (n <= 16) e = launch_rows<TI, TO, VEC, 16, false>(b, rows + at, n, stream);
+        else if (n <= 96) e = launch_rows<TI, TO, VEC, 96, false>(b, rows + at, n, stream);
+        else e = launch_rows<TI, TO, VEC, kBlockRows, false>(b, rows + at, n, stream);
         if (e != 0) return e;
         ++*launches;
     }
     return 0;
 }
 
+// Whether every row of both matrices starts on a boundary of VEC elements.
+template <class TI, class TO, int VEC>
+bool aligned(const AdjustArgs& a) {
+    constexpr size_t bi = sizeof(TI) * VEC, bo = sizeof(TO) * VEC;
+    return reinterpret_cast<uintptr_t>(a.in) % bi == 0 && a.ld * (int64_t)sizeof(TI) % (int64_t)bi == 0 && reinterpret_cast<uintptr_t>(a.out) % bo == 0 &&
+           a.out_ld * (int64_t)sizeof(TO) % (int64_t)bo == 0;
+}
 template <class TI, class TO>
 int launch_types(const AdjustArgs& a, const AdjustRow* rows, cudaStream_t stream, int* launches) {
-    // whole vectors where every row of both matrices starts on a vector's boundary
-    constexpr int kVec = 16 / sizeof(TI);
-    constexpr size_t out_bytes = std::min<size_t>(16, sizeof(TO) * kVec);
-    const bool aligned = reinterpret_cast<uintptr_t>(a.in) % 16 == 0 && a.ld * (int64_t)sizeof(TI) % 16 == 0 &&
-                         reinterpret_cast<uintptr_t>(a.out) % out_bytes == 0 && a.out_ld * (int64_t)sizeof(TO) % (int64_t)out_bytes == 0;
-    return aligned ? launch_vec<TI, TO, kVec>(a, rows, stream, launches) : launch_vec<TI, TO, 1>(a, rows, stream, launches);
+    if (aligned<TI, TO, 8>(a)) return launch_vec<TI, TO, 8>(a, rows, stream, launches);
+    if (aligned<TI, TO, 4>(a)) return launch_vec<TI, TO, 4>(a, rows, stream, launches);
+    return launch_vec<TI, TO, 1>(a, rows, stream, launches);
 }
 
 }  // namespace
