@@ -4,11 +4,11 @@
 // mantissa bits of a number between 16 and 32), tensor cores add up (16 + q) x in fp32 for one group on top of -24 times the
 // group's sum of x, and the scale is multiplied in fp32.  For up to 16 hidden states a pass the weights' bytes bound it.
 //
-// Layout (laid out once): tiles of 16 vocabulary rows, within a tile blocks of 64 weights a row, within a block 16 bytes per lane
-// of the warp that multiplies it.  Lane 4 g + t holds, of rows g and g + 8, the weights 8 t .. 8 t + 7 of the block's two halves
-// of 32: words (g, half 0), (g + 8, half 0), (g, half 1), (g + 8, half 1), each rotated left by three bits so that its first pair
-// of weights already lies where bf16 wants it.  A lane's word is one lane's part of an operand fragment, with the k of a half
-// taken in the order that makes it so; hidden states are put in the same order.
+// Layout (laid out once): pairs of tiles of 16 vocabulary rows; of a pair, block by block of 64 weights a row, 16 bytes per tile and
+// lane of the warp that multiplies it.  Lane 4 g + t holds, of rows g and g + 8 of the tile and of both halves (32 weights) of the
+// block, the weights 8 i + 2 t and 8 i + 2 t + 1, i = 0 .. 3: what an operand fragment wants of it.  Words (g, half 0), (g + 8, half 0),
+// (g, half 1), (g + 8, half 1); the bits of weight 8 i + 2 t stand at 4 i, those of its neighbour at 4 i + 16, the whole rotated left by
+// three bits so that pair 0 already lies where bf16 wants it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -22,51 +22,51 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kAhead = 4;                    // blocks of 64 weights that a warp has on their way
+#ifndef HEAD_AHEAD
+#define HEAD_AHEAD 4
+#endif
+constexpr int kAhead = HEAD_AHEAD;                    // blocks of 64 weights that a warp has on their way
 constexpr int kSharedMax = 227 * 1024;
 
-// Blocks of 64 weights a row is padded to, and 16-bit scales a lane's row pair needs per block.
+// Blocks of 64 weights a row is padded to, and bytes of a pair of tiles (32 rows): of weights, and of scales, which lie as
+// [block or pair of blocks][tile][g 0..7][...]: for groups of 32 the scales of (row g, half 0), (g + 8, 0), (g, 1), (g + 8, 1),
+// otherwise of (g), (g + 8) for the block's (128: the two blocks') group.
 __host__ __device__ constexpr int row_blocks(int n_hidden) { return (n_hidden + 63) / 64; }
-// Scales lie as [tile][block or pair of blocks][g 0..7][...]: for groups of 32 the lane's (row g, half 0), (g + 8, 0), (g, 1), (g + 8, 1),
-// otherwise (g), (g + 8) of the block's (128: of the two blocks') group.
-__host__ __device__ constexpr int scale_bytes_per_tile(int n_hidden, int group) {
-    return group == 32 ? row_blocks(n_hidden) * 64 : group == 64 ? row_blocks(n_hidden) * 32 : row_blocks(n_hidden) / 2 * 32;
+__host__ __device__ constexpr int64_t pair_weights(int n_hidden) { return (int64_t)row_blocks(n_hidden) * 1024; }
+__host__ __device__ constexpr int pair_scales(int n_hidden, int group) {
+    return group == 32 ? row_blocks(n_hidden) * 128 : group == 64 ? row_blocks(n_hidden) * 64 : row_blocks(n_hidden) / 2 * 64;
 }
+__host__ __device__ constexpr int64_t padded_pairs(int n_vocab) { return (int64_t)((n_vocab + 127) / 128) * 4; }
 
 // ------------------------------------------------------------------------------------------------ layout
 __global__ void layout_weights_kernel(const unsigned char* __restrict__ w, int n_vocab, int n_hidden, uint32_t* __restrict__ out) {
     const int blocks = row_blocks(n_hidden);
-    const int64_t words = (int64_t)((n_vocab + 127) / 128) * 8 * blocks * 128;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (int64_t)gridDim.x * blockDim.x) {
-        const int slot = (int)(i & 3), lane = (int)(i >> 2) & 31;
-        const int64_t tb = i >> 7;
-        const int block = (int)(tb % blocks);
-        const int64_t row = tb / blocks * 16 + (lane >> 2) + (slot & 1) * 8;
-        const int k = block * 64 + (slot >> 1) * 32 + (lane & 3) * 8;
+    const int64_t words = padded_pairs(n_vocab) * blocks * 256;
+    for (int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; n < words; n += (int64_t)gridDim.x * blockDim.x) {
+        const int slot = (int)(n & 3), lane = (int)(n >> 2) & 31, tile = (int)(n >> 7) & 1;
+        const int64_t pb = n >> 8;
+        const int block = (int)(pb % blocks);
+        const int64_t row = pb / blocks * 32 + tile * 16 + (lane >> 2) + (slot & 1) * 8;
+        const int k = block * 64 + (slot >> 1) * 32 + (lane & 3) * 2;
         uint32_t v = 0x88888888u;   // weights of value 0
         if (row < n_vocab && k < n_hidden) {
             const unsigned char* p = w + row * (n_hidden / 2) + k / 2;
-            v = (uint32_t)p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
+            v = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v |= (uint32_t)(p[4 * i] & 15) << (4 * i) | (uint32_t)(p[4 * i] >> 4) << (4 * i + 16);
         }
-        out[i] = __funnelshift_l(v, v, 3);
+        out[n] = __funnelshift_l(v, v, 3);
     }
 }
 __global__ void layout_scales_kernel(const unsigned short* __restrict__ s, int n_vocab, int n_hidden, int group, unsigned short* __restrict__ out) {
-    const int per_tile = scale_bytes_per_tile(n_hidden, group) / 2, groups = n_hidden / group;
-    const int64_t n = (int64_t)((n_vocab + 127) / 128) * 8 * per_tile;
+    const int per_pair = pair_scales(n_hidden, group) / 2, groups = n_hidden / group;
+    const int64_t n = padded_pairs(n_vocab) * per_pair;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int j = (int)(i % per_tile);
-        int g, r8, lane_row;
-        if (group == 32) {
-            g = (j >> 5) * 2 + (j >> 1 & 1);
-            lane_row = j >> 2 & 7;
-            r8 = j & 1;
-        } else {
-            g = j >> 4;
-            lane_row = j >> 1 & 7;
-            r8 = j & 1;
-        }
-        const int64_t row = i / per_tile * 16 + lane_row + r8 * 8;
+        const int j = (int)(i % per_pair);
+        const int per_tile = group == 32 ? 32 : 16, q = j / per_tile, in_tile = j % per_tile;
+        const int tile = q & 1, r8 = in_tile & 1;
+        const int g = group == 32 ? (q >> 1) * 2 + (in_tile >> 1 & 1) : q >> 1;
+        const int64_t row = i / per_pair * 32 + tile * 16 + r8 * 8 + (group == 32 ? in_tile >> 2 : in_tile >> 1);
         out[i] = row < n_vocab && g < groups ? s[row * groups + g] : (unsigned short)0;
     }
 }
@@ -79,23 +79,34 @@ struct HeadPlan {
     int vec;           // hidden states may be read 16 bytes at a time
 };
 
-// Two of a word's weights as 16-bit floats 16 + q: pair i holds weights i and i + 4 of the word's eight.
+// Two neighbouring weights as 16-bit floats 16 + q: pair i of a word.  The constants are handed over in registers: an instruction has
+// room for one of them only.
 template <class X>
-__device__ __forceinline__ uint32_t weight_pair(uint32_t w, int i) {
-    if constexpr (std::is_same<X, __nv_bfloat16>::value) return (__funnelshift_r(w, w, 4 * i) & 0x00780078u) | 0x41804180u;
-    else return (__funnelshift_r(w, w, (4 * i + 29) & 31) & 0x03C003C0u) | 0x4C004C00u;
-}
+struct Unpack {
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ Unpack() {
+        constexpr bool bf16 = std::is_same<X, __nv_bfloat16>::value;
+        asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(bf16 ? 0x00780078 : 0x03C003C0));
+        asm volatile("mov.b32 %0, %1;" : "=r"(sixteen) : "n"(bf16 ? 0x41804180 : 0x4C004C00));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int i) const {
+        const int turn = std::is_same<X, __nv_bfloat16>::value ? 4 * i : (4 * i + 29) & 31;
+        uint32_t v = __funnelshift_r(w, w, turn);
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(v), "r"(mask), "r"(sixteen));
+        return v;
+    }
+};
 
 template <class X>
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
     if constexpr (std::is_same<X, __nv_bfloat16>::value)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 __device__ __forceinline__ uint4 load_stream(const unsigned char* p) {
@@ -109,79 +120,86 @@ __device__ __forceinline__ float2 two_scales(uint32_t s, bool bf16) {
     return __half22float2(*reinterpret_cast<const __half2*>(&s));
 }
 
+template <class X>
+__device__ __forceinline__ float sum_of(uint32_t pair) {
+    if constexpr (std::is_same<X, __nv_bfloat16>::value) return __uint_as_float(pair << 16) + __uint_as_float(pair & 0xffff0000u);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    return f.x + f.y;
+}
+
 // GS: halves of 32 per group.  NT: eights of hidden states.
+// A warp works through units of 32 vocabulary rows and its share of their k, block by block, with kAhead blocks on their way in
+// registers: the weights go from memory to the tensor cores without touching shared memory.  The warps that share a unit add up
+// their parts in shared memory, in a fixed order.
 template <class X, int GS, int NT>
 __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant__ HeadPlan P) {
     extern __shared__ __align__(16) unsigned char smem[];
     const HeadArgs& a = P.a;
     constexpr int kBuffers = 2;
-    const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = (int)threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int blocks = row_blocks(a.n_hidden), ks = P.ksplit, kw = warp % ks, rg = warp / ks, groups_of_warps = kWarps / ks;
     const int m0 = (int)blockIdx.y * P.tokens, mt = min(P.tokens, a.n_rows - m0);
     // a warp's share of k, in pieces that hold whole groups
     constexpr int kPiece = GS == 4 ? 2 : 1;
     const int pieces = blocks / kPiece;
     const int p0 = pieces * kw / ks * kPiece, steps = pieces * (kw + 1) / ks * kPiece - p0;
-    const int pairs = (a.n_vocab + 31) / 32;                                  // tile pairs: 32 vocabulary rows
-    const int unit_stride = (int)gridDim.x * groups_of_warps;
-    const int first = (int)blockIdx.x * groups_of_warps + rg;
-    const int units = first < pairs ? (pairs - first + unit_stride - 1) / unit_stride : 0;
+    const int pairs = (a.n_vocab + 31) / 32;
+    const int stride = (int)gridDim.x * groups_of_warps, first = (int)blockIdx.x * groups_of_warps + rg;
 
     float* part = reinterpret_cast<float*>(smem);                              // [buffer][warp][8 NT][36]
     constexpr int kPart = NT * 8 * 36;
     float* xsum = part + kBuffers * kWarps * kPart;                            // [group][8 NT]: -24 times the group's sum
     const int groups = (2 * blocks + GS - 1) / GS;
-    unsigned char* xs = reinterpret_cast<unsigned char*>(xsum + groups * NT * 8);   // [half][hidden state][t] x 16 bytes
+    unsigned char* xs = reinterpret_cast<unsigned char*>(xsum + groups * NT * 8);   // [block][hidden state][2 halves][t] x 16 bytes
 
-    const size_t tile_w = (size_t)blocks * 512, tile_s = (size_t)scale_bytes_per_tile(a.n_hidden, 32 * GS);
-    constexpr int kScaleStep = GS == 1 ? 64 : 32;
-    // what is fetched next
-    int f_unit = 0, f_step = 0;
-    const unsigned char* f_w = a.weights + (size_t)first * 2 * tile_w + (size_t)p0 * 512 + lane * 16;
-    const unsigned char* f_s = a.scales + (size_t)first * 2 * tile_s + (size_t)(p0 / kPiece) * kScaleStep + g * (GS == 1 ? 8 : 4);
+    const int64_t tile_w = pair_weights(a.n_hidden), tile_s = pair_scales(a.n_hidden, 32 * GS);
+    constexpr int kScaleStep = GS == 1 ? 128 : 64;
+    const unsigned char* w_own = a.weights + p0 * 1024 + lane * 16;
+    const unsigned char* s_own = a.scales + p0 / kPiece * kScaleStep + g * (GS == 1 ? 8 : 4);
     uint4 w[kAhead][2];
     uint2 sc[kAhead][2];
-    auto fetch = [&](int i) {
-        if (f_unit >= units) return;
+    auto fetch = [&](int i, int pair, int step) {
+        const unsigned char* p = w_own + pair * tile_w + step * 1024;
+        const unsigned char* q = s_own + pair * tile_s + step / kPiece * kScaleStep;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            w[i][r] = load_stream(f_w + r * tile_w);
-            if constexpr (GS == 1) sc[i][r] = __ldg(reinterpret_cast<const uint2*>(f_s + r * tile_s));
-            else sc[i][r].x = __ldg(reinterpret_cast<const unsigned*>(f_s + r * tile_s));
-        }
-        ++f_step;
-        f_w += 512;
-        if (GS != 4 || (f_step & 1) == 0) f_s += kScaleStep;
-        if (f_step == steps) {
-            f_step = 0;
-            ++f_unit;
-            f_w += (size_t)unit_stride * 2 * tile_w - (size_t)steps * 512;
-            f_s += (size_t)unit_stride * 2 * tile_s - (size_t)(steps / kPiece) * kScaleStep;
+            w[i][r] = load_stream(p + r * 512);
+            if constexpr (GS == 1) sc[i][r] = __ldg(reinterpret_cast<const uint2*>(q + r * 64));
+            else sc[i][r].x = __ldg(reinterpret_cast<const unsigned*>(q + r * 32));
         }
     };
+    if (first < pairs) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(i);
+        for (int i = 0; i < kAhead; ++i)
+            if (i < steps) fetch(i, first, i);
+    }
 
-    // hidden states into shared memory, eight at a time, in the order of weight_pair
+    // Hidden states into shared memory: per half and lane t the pairs 8 i + 2 t, 16 bytes.  Odd states have their halves swapped, so
+    // that the lanes of a quarter warp read 128 different bytes of 128.
     const X* hidden = static_cast<const X*>(a.hidden);
-    for (int i = tid; i < mt * blocks * 8; i += kThreads) {
-        const int m = i / (blocks * 8), o = i - m * (blocks * 8);
-        const X* p = hidden + (int64_t)(m0 + m) * a.ld_hidden + o * 8;
-        alignas(16) unsigned short v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (o * 8 < a.n_hidden) {
-            if (P.vec) {
-                *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(p));
-            } else {
+    for (int i = tid; i < mt * blocks * 2; i += kThreads) {
+        const int m = i / (blocks * 2), h = i - m * (blocks * 2);
+        const X* p = hidden + (int64_t)(m0 + m) * a.ld_hidden + h * 32;
+        uint32_t v[16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __ldg(reinterpret_cast<const unsigned short*>(p) + j);
+        for (int j = 0; j < 16; ++j) v[j] = 0u;
+        if (h * 32 < a.n_hidden) {
+            if (P.vec) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + j);
+                    v[4 * j] = u.x, v[4 * j + 1] = u.y, v[4 * j + 2] = u.z, v[4 * j + 3] = u.w;
+                }
+            } else {
+                const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = (uint32_t)__ldg(e + 2 * j) | (uint32_t)__ldg(e + 2 * j + 1) << 16;
             }
         }
-        uint4 u;
-        u.x = (uint32_t)v[0] | (uint32_t)v[4] << 16;
-        u.y = (uint32_t)v[1] | (uint32_t)v[5] << 16;
-        u.z = (uint32_t)v[2] | (uint32_t)v[6] << 16;
-        u.w = (uint32_t)v[3] | (uint32_t)v[7] << 16;
-        *reinterpret_cast<uint4*>(xs + ((size_t)((o >> 2) * mt + m) * 4 + (o & 3)) * 16) = u;
+        uint4* to = reinterpret_cast<uint4*>(xs + ((size_t)(h >> 1) * mt + m) * 128 + ((h ^ m) & 1) * 64);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = make_uint4(v[j], v[4 + j], v[8 + j], v[12 + j]);
     }
     __syncthreads();
     for (int i = tid; i < groups * NT * 8; i += kThreads) {
@@ -189,92 +207,109 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         float sum = 0.0f;
         if (m < mt)
             for (int h = gr * GS; h < min(2 * blocks, gr * GS + GS); ++h) {
-                const X* p = reinterpret_cast<const X*>(xs + (size_t)(h * mt + m) * 64);
-#pragma unroll 8
-                for (int j = 0; j < 32; ++j) sum += (float)p[(j + 8 * (tid & 3)) & 31];
+                const uint4* p = reinterpret_cast<const uint4*>(xs + ((size_t)(h >> 1) * mt + m) * 128 + ((h ^ m) & 1) * 64);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 u = p[(j + tid) & 3];
+                    sum += sum_of<X>(u.x) + sum_of<X>(u.y) + (sum_of<X>(u.z) + sum_of<X>(u.w));
+                }
             }
         xsum[i] = -24.0f * sum;
     }
     __syncthreads();
 
-    float acc[2][NT][4];
+    // this lane's operand of the eights of hidden states; what has none takes another's, and nobody looks at the result
+    const unsigned char* xb[NT];
+    unsigned swap[NT];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.0f;
-    float d[2][NT][4];
+    for (int n = 0; n < NT; ++n) {
+        const int m = min(n * 8 + g, mt - 1);
+        xb[n] = xs + ((size_t)p0 * mt + m) * 128 + t * 16;
+        swap[n] = (m & 1) * 64;
+    }
+    const float* xc = xsum + p0 * 2 / GS * (NT * 8) + 2 * t;
     const bool bf16_scales = a.scale_type == FSB_BF16;
-    int unit = 0, step = 0;
-    while (unit < units) {
+    const Unpack<X> unpack;
+    int unit = 0;
+    for (int pair = first; pair < pairs; pair += stride, ++unit) {
+        float acc[2][NT][4], d[2][NT][4];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (unit >= units) break;
-            const int block = p0 + step;
-            float2 s[2][GS == 1 ? 2 : 1];
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                s[r][0] = two_scales(sc[i][r].x, bf16_scales);
-                if constexpr (GS == 1) s[r][1] = two_scales(sc[i][r].y, bf16_scales);
-            }
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const bool begins = GS == 1 || (half == 0 && (GS == 2 || (i & 1) == 0));
-                const bool ends = GS == 1 || (half == 1 && (GS == 2 || (i & 1) == 1));
+                for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.0f;
+        const bool more = pair + stride < pairs;
+        for (int step0 = 0; step0 < steps; step0 += kAhead) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint4 b = make_uint4(0u, 0u, 0u, 0u);
-                    if (n * 8 + g < mt) b = *reinterpret_cast<const uint4*>(xs + ((size_t)((block * 2 + half) * mt + n * 8 + g) * 4 + t) * 16);
-                    if (begins) {
-                        const float2 c = *reinterpret_cast<const float2*>(&xsum[(block * 2 + half) / GS * (NT * 8) + n * 8 + 2 * t]);
+            for (int i = 0; i < kAhead; ++i) {
+                const int step = step0 + i;
+                if (step >= steps) break;
+                float2 s[2][GS == 1 ? 2 : 1];
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) d[r][n][0] = d[r][n][2] = c.x, d[r][n][1] = d[r][n][3] = c.y;
-                    }
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint32_t lo = half ? w[i][r].z : w[i][r].x, hi = half ? w[i][r].w : w[i][r].y;
-                        mma<X>(d[r][n], weight_pair<X>(lo, 0), weight_pair<X>(hi, 0), weight_pair<X>(lo, 1), weight_pair<X>(hi, 1), b.x, b.y);
-                        mma<X>(d[r][n], weight_pair<X>(lo, 2), weight_pair<X>(hi, 2), weight_pair<X>(lo, 3), weight_pair<X>(hi, 3), b.z, b.w);
-                    }
-                    if (ends) {
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const float2 f = s[r][GS == 1 ? half : 0];
-                            acc[r][n][0] = fmaf(f.x, d[r][n][0], acc[r][n][0]);
-                            acc[r][n][1] = fmaf(f.x, d[r][n][1], acc[r][n][1]);
-                            acc[r][n][2] = fmaf(f.y, d[r][n][2], acc[r][n][2]);
-                            acc[r][n][3] = fmaf(f.y, d[r][n][3], acc[r][n][3]);
-                        }
-                    }
+                for (int r = 0; r < 2; ++r) {
+                    s[r][0] = two_scales(sc[i][r].x, bf16_scales);
+                    if constexpr (GS == 1) s[r][1] = two_scales(sc[i][r].y, bf16_scales);
                 }
-            }
-            fetch(i);
-            if (++step == steps) {   // the unit's 32 rows: the warps that share them add up their parts
-                float* to = part + ((unit & 1) * kWarps + warp) * kPart;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int half = 0; half < 2; ++half) {
+                    const bool begins = GS == 1 || (half == 0 && (GS == 2 || (i & 1) == 0));
+                    const bool ends = GS == 1 || (half == 1 && (GS == 2 || (i & 1) == 1));
+                    uint32_t p[2][8];
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int col = n * 8 + 2 * t + (j & 1);
-                            if (col < mt) to[col * 36 + r * 16 + g + (j >> 1) * 8] = acc[r][n][j];
-                            acc[r][n][j] = 0.0f;
+                            p[r][2 * j] = unpack.pair(half ? w[i][r].z : w[i][r].x, j);
+                            p[r][2 * j + 1] = unpack.pair(half ? w[i][r].w : w[i][r].y, j);
                         }
-                if (ks == 1) __syncwarp();
-                else asm volatile("bar.sync %0, %1;" ::"r"(1 + rg), "r"(32 * ks) : "memory");
-                const float* from = part + ((unit & 1) * kWarps + rg * ks) * kPart;
-                const int v0 = (first + unit * unit_stride) * 32;
-                for (int o = kw * 32 + lane; o < mt * 32; o += ks * 32) {
-                    const int col = o >> 5, row = o & 31;
-                    float sum = 0.0f;
-                    for (int q = 0; q < ks; ++q) sum += from[q * kPart + col * 36 + row];
-                    if (v0 + row < a.n_vocab) a.logits[(int64_t)(m0 + col) * a.ld + v0 + row] = sum;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint4 b = *reinterpret_cast<const uint4*>(xb[n] + step * mt * 128 + (swap[n] ^ (half * 64)));
+                        float2 c = make_float2(0.0f, 0.0f);
+                        if (begins) c = *reinterpret_cast<const float2*>(xc + (GS == 1 ? step * 2 + half : GS == 2 ? step : step / 2) * (NT * 8) + n * 8);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            if (begins) mma<X>(d[r][n], p[r][0], p[r][1], p[r][2], p[r][3], b.x, b.y, c.x, c.y, c.x, c.y);
+                            else mma<X>(d[r][n], p[r][0], p[r][1], p[r][2], p[r][3], b.x, b.y, d[r][n][0], d[r][n][1], d[r][n][2], d[r][n][3]);
+                            mma<X>(d[r][n], p[r][4], p[r][5], p[r][6], p[r][7], b.z, b.w, d[r][n][0], d[r][n][1], d[r][n][2], d[r][n][3]);
+                        }
+                        if (ends) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float2 f = s[r][GS == 1 ? half : 0];
+                                acc[r][n][0] = fmaf(f.x, d[r][n][0], acc[r][n][0]);
+                                acc[r][n][1] = fmaf(f.x, d[r][n][1], acc[r][n][1]);
+                                acc[r][n][2] = fmaf(f.y, d[r][n][2], acc[r][n][2]);
+                                acc[r][n][3] = fmaf(f.y, d[r][n][3], acc[r][n][3]);
+                            }
+                        }
+                    }
                 }
-                step = 0;
-                ++unit;
+                // the block that takes this one's place: four steps on, or of the next unit (every place is used last once)
+                if (step + kAhead < steps) fetch(i, pair, step + kAhead);
+                else if (more) fetch(i, pair + stride, i);
             }
+        }
+        // the warps that share these 32 rows add up their parts
+        float* to = part + ((unit & 1) * kWarps + warp) * kPart;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = n * 8 + 2 * t + (j & 1);
+                    if (col < mt) to[col * 36 + r * 16 + g + (j >> 1) * 8] = acc[r][n][j];
+                }
+        if (ks == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + rg), "r"(32 * ks) : "memory");
+        const float* from = part + ((unit & 1) * kWarps + rg * ks) * kPart + lane;
+        const int v = pair * 32 + lane;
+        for (int col = kw; col < mt; col += ks) {
+            float sum = 0.0f;
+            for (int q = 0; q < ks; ++q) sum += from[q * kPart + col * 36];
+            if (v < a.n_vocab) a.logits[(int64_t)(m0 + col) * a.ld + v] = sum;
         }
     }
 }
@@ -321,8 +356,8 @@ int prepare_head_kernels() {
     return e ? e : prepare_type<__half>();
 }
 
-int64_t head_weight_bytes(int n_vocab, int n_hidden) { return (int64_t)((n_vocab + 127) / 128) * 8 * row_blocks(n_hidden) * 512; }
-int64_t head_scale_bytes(int n_vocab, int n_hidden, int group) { return (int64_t)((n_vocab + 127) / 128) * 8 * scale_bytes_per_tile(n_hidden, group); }
+int64_t head_weight_bytes(int n_vocab, int n_hidden) { return padded_pairs(n_vocab) * pair_weights(n_hidden); }
+int64_t head_scale_bytes(int n_vocab, int n_hidden, int group) { return padded_pairs(n_vocab) * pair_scales(n_hidden, group); }
 
 int launch_head_layout(const unsigned char* weights, const void* scales, int n_vocab, int n_hidden, int group, unsigned char* weights_out,
                        unsigned char* scales_out, void* stream) {
