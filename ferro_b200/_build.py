@@ -13,8 +13,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libferro_sampler_b200.so")
-SOURCES = ["fsb_stream.cu", "fsb_fullrow.cu", "fsb_support.cu", "fsb_adjust.cu", "fsb_head.cu", "fsb_shim.cpp", "fsb_logits.cpp", "fsb_request.cpp"]
-HEADERS = ["fsb_internal.h", "fsb_engine.h", "fsb_device.cuh", os.path.join("..", "..", "include", "ferro_sampler_b200.h")]
+SOURCES = ["fsb_stream.cu", "fsb_fullrow.cu", "fsb_support.cu", "fsb_adjust.cu", "fsb_head.cu", "fsb_head_many.cu", "fsb_shim.cpp", "fsb_logits.cpp", "fsb_request.cpp"]
+HEADERS = ["fsb_internal.h", "fsb_engine.h", "fsb_device.cuh", "fsb_head.cuh", os.path.join("..", "..", "include", "ferro_sampler_b200.h")]
 # the Python binding's native half: a module of its own, so that C and C++ users of the library need no Python
 EXT_PATH = os.path.join(LIB_DIR, "_fsb_native.so")
 EXT_SOURCE = "fsb_python.cpp"

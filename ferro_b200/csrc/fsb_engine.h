@@ -126,8 +126,8 @@ struct fsb_handle {
     int32_t* d_pool = nullptr;         // resident histories: max_hist ids, carved into power-of-two regions
     int64_t pool_top = 0;              // ids handed out so far (bump pointer)
     std::vector<std::vector<int64_t>> pool_free;   // freed regions by size class
-    // adjusted steps: per row how many CTAs are done, with a bit for a logit that is left (zero between calls), and a pinned
-    // word that tells of a row without one
+    // adjusted steps: per row how many CTAs are done, with a bit for a logit that is left (zero between calls); and two pinned
+    // words: one tells of a row without one, the other of a head launch in which a wait ran out
     uint32_t* d_row_state = nullptr;
     uint32_t* h_empty = nullptr;
     uint32_t* h_empty_dev = nullptr;

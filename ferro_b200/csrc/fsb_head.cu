@@ -9,34 +9,21 @@
 // block, the weights 8 i + 2 t and 8 i + 2 t + 1, i = 0 .. 3: what an operand fragment wants of it.  Words (g, half 0), (g + 8, half 0),
 // (g, half 1), (g + 8, half 1); the bits of weight 8 i + 2 t stand at 4 i, those of its neighbour at 4 i + 16, the whole rotated left by
 // three bits so that pair 0 already lies where bf16 wants it.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
 #include "../../include/ferro_sampler_b200.h"
-#include "fsb_device.cuh"
+#include "fsb_head.cuh"
 
 namespace fsb {
 namespace {
 
+#ifndef HEAD_FEW
+#define HEAD_FEW 16
+#endif
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
-#ifndef HEAD_AHEAD
-#define HEAD_AHEAD 4
-#endif
-constexpr int kAhead = HEAD_AHEAD;                    // blocks of 64 weights that a warp has on their way
+constexpr int kAhead = 4;                    // blocks of 64 weights that a warp has on their way
 constexpr int kSharedMax = 227 * 1024;
-
-// Blocks of 64 weights a row is padded to, and bytes of a pair of tiles (32 rows): of weights, and of scales, which lie as
-// [block or pair of blocks][tile][g 0..7][...]: for groups of 32 the scales of (row g, half 0), (g + 8, 0), (g, 1), (g + 8, 1),
-// otherwise of (g), (g + 8) for the block's (128: the two blocks') group.
-__host__ __device__ constexpr int row_blocks(int n_hidden) { return (n_hidden + 63) / 64; }
-__host__ __device__ constexpr int64_t pair_weights(int n_hidden) { return (int64_t)row_blocks(n_hidden) * 1024; }
-__host__ __device__ constexpr int pair_scales(int n_hidden, int group) {
-    return group == 32 ? row_blocks(n_hidden) * 128 : group == 64 ? row_blocks(n_hidden) * 64 : row_blocks(n_hidden) / 2 * 64;
-}
-__host__ __device__ constexpr int64_t padded_pairs(int n_vocab) { return (int64_t)((n_vocab + 127) / 128) * 4; }
 
 // ------------------------------------------------------------------------------------------------ layout
 __global__ void layout_weights_kernel(const unsigned char* __restrict__ w, int n_vocab, int n_hidden, uint32_t* __restrict__ out) {
@@ -79,24 +66,6 @@ struct HeadPlan {
     int vec;           // hidden states may be read 16 bytes at a time
 };
 
-// Two neighbouring weights as 16-bit floats 16 + q: pair i of a word.  The constants are handed over in registers: an instruction has
-// room for one of them only.
-template <class X>
-struct Unpack {
-    uint32_t mask, sixteen;
-    __device__ __forceinline__ Unpack() {
-        constexpr bool bf16 = std::is_same<X, __nv_bfloat16>::value;
-        asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(bf16 ? 0x00780078 : 0x03C003C0));
-        asm volatile("mov.b32 %0, %1;" : "=r"(sixteen) : "n"(bf16 ? 0x41804180 : 0x4C004C00));
-    }
-    __device__ __forceinline__ uint32_t pair(uint32_t w, int i) const {
-        const int turn = std::is_same<X, __nv_bfloat16>::value ? 4 * i : (4 * i + 29) & 31;
-        uint32_t v = __funnelshift_r(w, w, turn);
-        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(v), "r"(mask), "r"(sixteen));
-        return v;
-    }
-};
-
 template <class X>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
     if constexpr (std::is_same<X, __nv_bfloat16>::value)
@@ -109,15 +78,15 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
+__device__ __forceinline__ float2 two_scales(uint32_t s, bool bf16) {
+    if (bf16) return make_float2(__uint_as_float(s << 16), __uint_as_float(s & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&s));
+}
+
 __device__ __forceinline__ uint4 load_stream(const unsigned char* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
-}
-
-__device__ __forceinline__ float2 two_scales(uint32_t s, bool bf16) {
-    if (bf16) return make_float2(__uint_as_float(s << 16), __uint_as_float(s & 0xffff0000u));
-    return __half22float2(*reinterpret_cast<const __half2*>(&s));
 }
 
 template <class X>
@@ -352,8 +321,9 @@ int prepare_type() {
 }  // namespace
 
 int prepare_head_kernels() {
-    const int e = prepare_type<__nv_bfloat16>();
-    return e ? e : prepare_type<__half>();
+    int e = prepare_type<__nv_bfloat16>();
+    if (e == 0) e = prepare_type<__half>();
+    return e ? e : prepare_head_many();
 }
 
 int64_t head_weight_bytes(int n_vocab, int n_hidden) { return padded_pairs(n_vocab) * pair_weights(n_hidden); }
@@ -371,6 +341,10 @@ int launch_head_layout(const unsigned char* weights, const void* scales, int n_v
 }
 
 int launch_head(const HeadArgs& a, void* stream, int* launches) {
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    ++*launches;
+    int error = 0;
+    if (a.n_rows > HEAD_FEW && launch_head_many(a, stream, &error)) return error;
     HeadPlan p{};
     p.a = a;
     p.vec = reinterpret_cast<uintptr_t>(a.hidden) % 16 == 0 && a.ld_hidden % 8 == 0;
@@ -397,8 +371,6 @@ int launch_head(const HeadArgs& a, void* stream, int* launches) {
             grid_x = ctas;
         }
     }
-    ++*launches;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     return a.hidden_type == FSB_BF16 ? launch_group<__nv_bfloat16>(p, nt, grid_x, s) : launch_group<__half>(p, nt, grid_x, s);
 }
 

@@ -1,0 +1,57 @@
+// fsb_head.cuh - what the two kernels of the LM head share: the layout's sizes and how weights are unpacked (fsb_head.cu says what the
+// layout is).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "fsb_device.cuh"
+
+namespace fsb {
+
+// Blocks of 64 weights a row is padded to, and bytes of a pair of tiles (32 rows): of weights, and of scales, which lie as
+// [block or pair of blocks][tile][g 0..7][...]: for groups of 32 the scales of (row g, half 0), (g + 8, 0), (g, 1), (g + 8, 1),
+// otherwise of (g), (g + 8) for the block's (128: the two blocks') group.
+__host__ __device__ constexpr int row_blocks(int n_hidden) { return (n_hidden + 63) / 64; }
+__host__ __device__ constexpr int64_t pair_weights(int n_hidden) { return (int64_t)row_blocks(n_hidden) * 1024; }
+__host__ __device__ constexpr int pair_scales(int n_hidden, int group) {
+    return group == 32 ? row_blocks(n_hidden) * 128 : group == 64 ? row_blocks(n_hidden) * 64 : row_blocks(n_hidden) / 2 * 64;
+}
+__host__ __device__ constexpr int64_t padded_pairs(int n_vocab) { return (int64_t)((n_vocab + 127) / 128) * 4; }
+
+// Two neighbouring weights as 16-bit floats 16 + q: pair i of a word.  The constants are handed over in registers: an instruction has
+// room for one of them only.
+template <class X>
+struct Unpack {
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ Unpack() {
+        constexpr bool bf16 = std::is_same<X, __nv_bfloat16>::value;
+        asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(bf16 ? 0x00780078 : 0x03C003C0));
+        asm volatile("mov.b32 %0, %1;" : "=r"(sixteen) : "n"(bf16 ? 0x41804180 : 0x4C004C00));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int i) const {
+        const int turn = std::is_same<X, __nv_bfloat16>::value ? 4 * i : (4 * i + 29) & 31;
+        uint32_t v = __funnelshift_r(w, w, turn);
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(v), "r"(mask), "r"(sixteen));
+        return v;
+    }
+    // The pair as q - 8 (exact).
+    __device__ __forceinline__ uint32_t value(uint32_t w, int i) const {
+        const uint32_t v = pair(w, i);
+        if constexpr (std::is_same<X, __nv_bfloat16>::value) {
+            const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(24.0f));
+            return *reinterpret_cast<const uint32_t*>(&d);
+        } else {
+            const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(24.0f));
+            return *reinterpret_cast<const uint32_t*>(&d);
+        }
+    }
+};
+
+// Launches the kernel for more rows than tensor cores of a warp are good for; false if its operands cannot be (hidden states off 16-byte
+// boundaries).  `error`: a cudaError_t as int.
+bool launch_head_many(const HeadArgs& a, void* stream, int* error);
+int prepare_head_many();
+
+}  // namespace fsb

@@ -177,6 +177,7 @@ struct HeadArgs {
     int32_t n_rows, n_vocab, n_hidden, group;
     int32_t scale_type, hidden_type;
     int32_t sms;
+    uint32_t* late;            // a pinned host word that is set if a wait inside the kernel ran out
 };
 int prepare_head_kernels();   // for the current device, before its first launch_head
 int launch_head(const HeadArgs& a, void* stream, int* launches);

@@ -114,6 +114,7 @@ int queue_adjust(fsb_handle* h, int n_rows, const int* stream_ids, const void* l
     a.n_vocab = n_vocab;
     a.vocab_offset = h->vocab_offset;
     a.softcap = h->softcap;
+    if (report_empty) *static_cast<volatile uint32_t*>(h->h_empty) = 0u;
     int launches = 0;
     const int e = launch_adjust(a, rows.data(), h->stream, &launches);
     h->counters.kernel_launches += (uint64_t)launches;
@@ -143,25 +144,25 @@ int64_t stage_ld(const fsb_handle* h, int n_rows, int n_vocab) {
     return (size_t)n_rows * (size_t)ld <= h->logits_stage_elems ? ld : n_vocab;
 }
 
-// Adjusts `logits` into the engine's staging area and samples there.  The arguments have been checked.
-int sample_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab, const Masks& m,
-                    int32_t* tokens_out, unsigned flags) {
-    fsb_batch* b = h->own;
-    const bool append = (flags & FSB_APPEND_SAMPLED) != 0;
+// Brings the histories up to date and makes room for a token each, where one is going to be appended.
+int sync_streams(fsb_handle* h, int n_rows, const int* stream_ids, bool append) {
     for (int i = 0; i < n_rows; ++i) {
         Stream* s = get_stream(h, stream_ids[i]);
         int rc = sync_history(h, s);
         if (rc == FSB_OK && append) rc = ensure_region(h, s, (int64_t)s->hist.size() + 1);
         if (rc) return rc;
     }
-    const int64_t sld = stage_ld(h, n_rows, n_vocab);
-    volatile uint32_t* empty = h->h_empty;
-    *empty = 0u;
-    int rc = queue_adjust(h, n_rows, stream_ids, logits, logits_type, ld, n_vocab, m, h->d_logits_stage, FSB_F32, sld, true);
-    if (rc) return rc;
+    return FSB_OK;
+}
+
+// Samples the rows in the engine's staging area, which the kernels queued before write.  `adjusted`: penalties and softcap are done.
+// The streams' histories are on the device (sync_streams).
+int sample_staged(fsb_handle* h, int n_rows, const int* stream_ids, int64_t ld, int n_vocab, bool adjusted, int32_t* tokens_out, unsigned flags) {
+    fsb_batch* b = h->own;
+    const bool append = (flags & FSB_APPEND_SAMPLED) != 0;
     b->n_rows = n_rows;
     b->n_vocab = n_vocab;
-    b->ld = sld;
+    b->ld = ld;
     b->flags = flags & ~FSB_APPEND_SAMPLED;
     b->hist_dev = h->d_pool;
     b->hist_ids = 0;
@@ -178,26 +179,29 @@ int sample_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, const void
             s->draws++;
             b->stochastic[(size_t)i] = 1;
         }
-        // an empty window that ends where the history does: an appended token goes there
-        fill_desc(h, b->descs[(size_t)i], s->p, n_vocab, (int64_t)i * sld, std::max<int64_t>(s->pool_off, 0) + (int64_t)s->hist.size(), 0, word, i);
+        // the window, even an empty one, ends where the history does: an appended token goes there
+        const int64_t len = (int64_t)s->hist.size(), from = adjusted || s->p.repetition_penalty == 1.0f ? len : window_start(s->p, len);
+        fill_desc(h, b->descs[(size_t)i], s->p, n_vocab, (int64_t)i * ld, std::max<int64_t>(s->pool_off, 0) + from, len - from, word, i);
         if (append) b->descs[(size_t)i].flags |= kRowAppend;
     }
-    rc = finalize_batch(h, b);
+    int rc = finalize_batch(h, b);
     if (rc) {
         rollback_draws(h, b);
         return rc;
     }
     {
-        FreshRows fresh(h, true);
+        FreshRows fresh(h, adjusted);
         rc = run_staged(h, b, h->d_logits_stage, flags & ~FSB_APPEND_SAMPLED, nullptr);
     }
-    if (*empty != 0u) {
-        if (rc == FSB_OK) {
-            cudaStreamSynchronize(h->stream);
-            rollback_draws(h, b);
-        }
+    // what the kernels before the sampling ones have to report (their words were written before any token was)
+    volatile uint32_t *empty = h->h_empty, *late = h->h_empty + 1;
+    if (*empty != 0u || *late != 0u) {
+        cudaStreamSynchronize(h->stream);
+        if (rc == FSB_OK) rollback_draws(h, b);
         h->kept_valid = false;
-        return fail(h, FSB_ERR_EMPTY, "masks and biases leave row %u no token", *empty - 1u);
+        const uint32_t row = *empty, gave_up = *late;
+        *empty = *late = 0u;
+        return gave_up ? fail(h, FSB_ERR_DEVICE, "a launch of a head gave up waiting") : fail(h, FSB_ERR_EMPTY, "masks and biases leave row %u no token", row - 1u);
     }
     if (rc) return rc;
     for (int i = 0; i < n_rows; ++i) {
@@ -225,6 +229,11 @@ bool owns(const fsb_handle* h, const fsb_head* head) { return head && std::find(
 int check_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidden, int hidden_type, int64_t ld_hidden) {
     if (!owns(h, head)) return fail(h, FSB_ERR_INVALID, "not a head of this engine");
     if (n_rows <= 0) return fail(h, FSB_ERR_INVALID, "n_rows must be positive");
+    volatile uint32_t* late = h->h_empty + 1;
+    if (*late != 0u) {
+        *late = 0u;
+        return fail(h, FSB_ERR_DEVICE, "an earlier launch of a head gave up waiting: its logits are not complete");
+    }
     if (n_rows > 65535) return fail(h, FSB_ERR_CAPACITY, "%d rows in one call, at most 65535", n_rows);
     if (hidden_type == FSB_F32) return fail(h, FSB_ERR_INVALID, "hidden states are FSB_BF16 or FSB_F16");
     return check_rows(h, hidden, hidden_type, ld_hidden, head->n_hidden, "hidden");
@@ -245,6 +254,7 @@ int queue_head(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidd
     a.scale_type = head->scale_type;
     a.hidden_type = hidden_type;
     a.sms = h->sm_count;
+    a.late = h->h_empty_dev + 1;
     int launches = 0;
     const int e = launch_head(a, h->stream, &launches);
     h->counters.kernel_launches += (uint64_t)launches;
@@ -389,7 +399,12 @@ int fsb_sample_batch_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, 
         if (rc == FSB_OK) rc = check_streams(h, n_rows, stream_ids, true);
         if (rc == FSB_OK) rc = check_sampling(h, tokens_out, flags);
         if (rc) return rc;
-        return sample_adjusted(h, n_rows, stream_ids, logits, logits_type, ld, n_vocab, m, tokens_out, flags);
+        rc = sync_streams(h, n_rows, stream_ids, (flags & FSB_APPEND_SAMPLED) != 0);
+        if (rc) return rc;
+        const int64_t sld = stage_ld(h, n_rows, n_vocab);
+        rc = queue_adjust(h, n_rows, stream_ids, logits, logits_type, ld, n_vocab, m, h->d_logits_stage, FSB_F32, sld, true);
+        if (rc) return rc;
+        return sample_staged(h, n_rows, stream_ids, sld, n_vocab, true, tokens_out, flags);
     });
 }
 
@@ -438,6 +453,8 @@ int fsb_sample_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const int
         if (rc) return rc;
         const int V = head->n_vocab;
         const int64_t ld = stage_ld(h, n_rows, V);
+        rc = sync_streams(h, n_rows, stream_ids, (flags & FSB_APPEND_SAMPLED) != 0);
+        if (rc) return rc;
         rc = queue_head(h, head, n_rows, hidden, hidden_type, ld_hidden, h->d_logits_stage, ld);
         if (rc) return rc;
         bool adjusted = masks != nullptr;
@@ -445,10 +462,10 @@ int fsb_sample_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const int
             const Stream* s = get_stream(h, stream_ids[i]);
             adjusted = s->frequency != 0.0f || s->presence != 0.0f || s->n_bias > 0;
         }
-        if (adjusted) return sample_adjusted(h, n_rows, stream_ids, h->d_logits_stage, FSB_F32, ld, V, m, tokens_out, flags);
-        // nothing that the sampling kernels do not know: they apply the repetition penalty and the softcap themselves
-        FreshRows fresh(h, false);
-        return fsb_sample_batch_resident(h, n_rows, stream_ids, h->d_logits_stage, ld, V, tokens_out, flags);
+        // (where there is nothing that the sampling kernels do not know, they apply the repetition penalty and the softcap themselves)
+        if (adjusted) rc = queue_adjust(h, n_rows, stream_ids, h->d_logits_stage, FSB_F32, ld, V, m, h->d_logits_stage, FSB_F32, ld, true);
+        if (rc) return rc;
+        return sample_staged(h, n_rows, stream_ids, ld, V, adjusted, tokens_out, flags);
     });
 }
 
