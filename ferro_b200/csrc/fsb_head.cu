@@ -4,11 +4,12 @@
 // mantissa bits of a number between 16 and 32), tensor cores add up (16 + q) x in fp32 for one group on top of -24 times the
 // group's sum of x, and the scale is multiplied in fp32.  For up to 16 hidden states a pass the weights' bytes bound it.
 //
-// Layout (laid out once): pairs of tiles of 16 vocabulary rows; of a pair, block by block of 64 weights a row, 16 bytes per tile and
-// lane of the warp that multiplies it.  Lane 4 g + t holds, of rows g and g + 8 of the tile and of both halves (32 weights) of the
-// block, the weights 8 i + 2 t and 8 i + 2 t + 1, i = 0 .. 3: what an operand fragment wants of it.  Words (g, half 0), (g + 8, half 0),
-// (g, half 1), (g + 8, half 1); the bits of weight 8 i + 2 t stand at 4 i, those of its neighbour at 4 i + 16, the whole rotated left by
-// three bits so that pair 0 already lies where bf16 wants it.
+// Layout (laid out once): units of eight pairs of tiles of 16 vocabulary rows; of a unit block by block of 64 weights a row, pair by
+// pair, 16 bytes per tile and lane of the warp that multiplies it.  Lane 4 g + t holds, of rows g and g + 8 of the tile and of both halves
+// (32 weights) of the block, the weights 8 i + 2 t and 8 i + 2 t + 1, i = 0 .. 3: what an operand fragment wants of it.  Words (g, half
+// 0), (g + 8, half 0), (g, half 1), (g + 8, half 1); the bits of weight 8 i + 2 t stand at 4 i, those of its neighbour at 4 i + 16, the
+// whole rotated left by three bits so that pair 0 already lies where bf16 wants it.  Scales of a pair and block, tile by tile: for groups
+// of 32 [g][half][row g, row g + 8], otherwise [g][row g, row g + 8].
 #include <algorithm>
 
 #include "../../include/ferro_sampler_b200.h"
@@ -28,12 +29,12 @@ constexpr int kSharedMax = 227 * 1024;
 // ------------------------------------------------------------------------------------------------ layout
 __global__ void layout_weights_kernel(const unsigned char* __restrict__ w, int n_vocab, int n_hidden, uint32_t* __restrict__ out) {
     const int blocks = row_blocks(n_hidden);
-    const int64_t words = padded_pairs(n_vocab) * blocks * 256;
+    const int64_t words = head_units(n_vocab) * blocks * 2048;
     for (int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; n < words; n += (int64_t)gridDim.x * blockDim.x) {
-        const int slot = (int)(n & 3), lane = (int)(n >> 2) & 31, tile = (int)(n >> 7) & 1;
-        const int64_t pb = n >> 8;
-        const int block = (int)(pb % blocks);
-        const int64_t row = pb / blocks * 32 + tile * 16 + (lane >> 2) + (slot & 1) * 8;
+        const int slot = (int)(n & 3), lane = (int)(n >> 2) & 31, tile = (int)(n >> 7) & 15;   // (of the unit's sixteen)
+        const int64_t ub = n >> 11;
+        const int block = (int)(ub % blocks);
+        const int64_t row = ub / blocks * 256 + tile * 16 + (lane >> 2) + (slot & 1) * 8;
         const int k = block * 64 + (slot >> 1) * 32 + (lane & 3) * 2;
         uint32_t v = 0x88888888u;   // weights of value 0
         if (row < n_vocab && k < n_hidden) {
@@ -46,14 +47,14 @@ __global__ void layout_weights_kernel(const unsigned char* __restrict__ w, int n
     }
 }
 __global__ void layout_scales_kernel(const unsigned short* __restrict__ s, int n_vocab, int n_hidden, int group, unsigned short* __restrict__ out) {
-    const int per_pair = pair_scales(n_hidden, group) / 2, groups = n_hidden / group;
-    const int64_t n = padded_pairs(n_vocab) * per_pair;
+    const int per_tile = scale_bytes(group) / 4, blocks = scale_blocks(n_hidden, group), groups = n_hidden / group;
+    const int64_t n = head_units(n_vocab) * blocks * 16 * per_tile;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int j = (int)(i % per_pair);
-        const int per_tile = group == 32 ? 32 : 16, q = j / per_tile, in_tile = j % per_tile;
-        const int tile = q & 1, r8 = in_tile & 1;
-        const int g = group == 32 ? (q >> 1) * 2 + (in_tile >> 1 & 1) : q >> 1;
-        const int64_t row = i / per_pair * 32 + tile * 16 + r8 * 8 + (group == 32 ? in_tile >> 2 : in_tile >> 1);
+        const int in_tile = (int)(i % per_tile), tile = (int)(i / per_tile) & 15;
+        const int64_t ub = i / (per_tile * 16);
+        const int block = (int)(ub % blocks);
+        const int g = group == 32 ? block * 2 + (in_tile >> 1 & 1) : block;
+        const int64_t row = ub / blocks * 256 + tile * 16 + (in_tile & 1) * 8 + (group == 32 ? in_tile >> 2 : in_tile >> 1);
         out[i] = row < n_vocab && g < groups ? s[row * groups + g] : (unsigned short)0;
     }
 }
@@ -122,15 +123,14 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
     const int groups = (2 * blocks + GS - 1) / GS;
     unsigned char* xs = reinterpret_cast<unsigned char*>(xsum + groups * NT * 8);   // [block][hidden state][2 halves][t] x 16 bytes
 
-    const int64_t tile_w = pair_weights(a.n_hidden), tile_s = pair_scales(a.n_hidden, 32 * GS);
-    constexpr int kScaleStep = GS == 1 ? 128 : 64;
-    const unsigned char* w_own = a.weights + p0 * 1024 + lane * 16;
-    const unsigned char* s_own = a.scales + p0 / kPiece * kScaleStep + g * (GS == 1 ? 8 : 4);
+    const int64_t unit_w = (int64_t)blocks * 8192, unit_s = (int64_t)scale_blocks(a.n_hidden, 32 * GS) * 8 * scale_bytes(32 * GS);
+    const unsigned char* w_own = a.weights + p0 * 8192 + lane * 16;
+    const unsigned char* s_own = a.scales + p0 / kPiece * 8 * scale_bytes(32 * GS) + g * (GS == 1 ? 8 : 4);
     uint4 w[kAhead][2];
     uint2 sc[kAhead][2];
     auto fetch = [&](int i, int pair, int step) {
-        const unsigned char* p = w_own + pair * tile_w + step * 1024;
-        const unsigned char* q = s_own + pair * tile_s + step / kPiece * kScaleStep;
+        const unsigned char* p = w_own + (pair >> 3) * unit_w + ((pair & 7) * 1024 + step * 8192);
+        const unsigned char* q = s_own + (pair >> 3) * unit_s + ((pair & 7) + step / kPiece * 8) * scale_bytes(32 * GS);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             w[i][r] = load_stream(p + r * 512);
@@ -326,8 +326,8 @@ int prepare_head_kernels() {
     return e ? e : prepare_head_many();
 }
 
-int64_t head_weight_bytes(int n_vocab, int n_hidden) { return padded_pairs(n_vocab) * pair_weights(n_hidden); }
-int64_t head_scale_bytes(int n_vocab, int n_hidden, int group) { return padded_pairs(n_vocab) * pair_scales(n_hidden, group); }
+int64_t head_weight_bytes(int n_vocab, int n_hidden) { return head_units(n_vocab) * row_blocks(n_hidden) * 8192; }
+int64_t head_scale_bytes(int n_vocab, int n_hidden, int group) { return head_units(n_vocab) * scale_blocks(n_hidden, group) * 8 * scale_bytes(group); }
 
 int launch_head_layout(const unsigned char* weights, const void* scales, int n_vocab, int n_hidden, int group, unsigned char* weights_out,
                        unsigned char* scales_out, void* stream) {

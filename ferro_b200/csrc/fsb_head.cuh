@@ -10,15 +10,12 @@
 
 namespace fsb {
 
-// Blocks of 64 weights a row is padded to, and bytes of a pair of tiles (32 rows): of weights, and of scales, which lie as
-// [block or pair of blocks][tile][g 0..7][...]: for groups of 32 the scales of (row g, half 0), (g + 8, 0), (g, 1), (g + 8, 1),
-// otherwise of (g), (g + 8) for the block's (128: the two blocks') group.
+// Blocks of 64 weights a row is padded to; tile pairs (32 vocabulary rows), eight of which make a unit.  Weights lie as [unit][block][pair]
+// x 1024 bytes, scales as [unit][block, for groups of 128 pair of blocks][pair] x scale_bytes.
 __host__ __device__ constexpr int row_blocks(int n_hidden) { return (n_hidden + 63) / 64; }
-__host__ __device__ constexpr int64_t pair_weights(int n_hidden) { return (int64_t)row_blocks(n_hidden) * 1024; }
-__host__ __device__ constexpr int pair_scales(int n_hidden, int group) {
-    return group == 32 ? row_blocks(n_hidden) * 128 : group == 64 ? row_blocks(n_hidden) * 64 : row_blocks(n_hidden) / 2 * 64;
-}
-__host__ __device__ constexpr int64_t padded_pairs(int n_vocab) { return (int64_t)((n_vocab + 127) / 128) * 4; }
+__host__ __device__ constexpr int scale_bytes(int group) { return group == 32 ? 128 : 64; }
+__host__ __device__ constexpr int scale_blocks(int n_hidden, int group) { return group == 128 ? row_blocks(n_hidden) / 2 : row_blocks(n_hidden); }
+__host__ __device__ constexpr int64_t head_units(int n_vocab) { return (n_vocab + 255) / 256; }
 
 // Two neighbouring weights as 16-bit floats 16 + q: pair i of a word.  The constants are handed over in registers: an instruction has
 // room for one of them only.
