@@ -2,7 +2,7 @@
 // the weights as operand A in tensor memory, unpacked there by the warps that later take the sums out again.
 //
 // A CTA takes 256 vocabulary rows at a time, in two halves, and all hidden states of the pass (up to 96).  Warps have one part each:
-// eight unpack weights (32 rows each, a block of 64 weights at a time) to q - 8 in bf16 / fp16, which is exact, and store them to tensor
+// sixteen unpack weights (32 rows of every second block of 64 weights each) to q - 8 in bf16 / fp16, which is exact, and store them to tensor
 // memory as 32 columns of pairs; two issue the products of 128 rows; eight take the sums of one group of weights out again, a thread
 // for every row and a register for every hidden state, and add them up times the row's scale, two to an instruction; one has weights
 // and hidden states copied into a ring of stages of two blocks.
@@ -16,7 +16,7 @@
 namespace fsb {
 namespace {
 
-constexpr int kManyThreads = 640;        // warps 0 - 7 take sums out, 8 - 15 unpack, 16 and 17 issue, 18 copies, 19 completes their group of four
+constexpr int kManyThreads = 896;        // warps 0 - 7 take sums out, 8 - 23 unpack, 24 and 25 issue, 26 copies, 27 completes their group of four
 constexpr int kRows = 256;               // vocabulary rows of a unit
 constexpr int kTokensMax = 96;
 constexpr int kSharedMax = 227 * 1024;
@@ -77,19 +77,21 @@ __device__ __forceinline__ void tc_store(unsigned addr, const uint32_t (&r)[16])
                  "r"(r[15])
                  : "memory");
 }
-// COLS columns of the warp's 32 lanes, waited for: nobody reads the registers earlier.
-template <int COLS>
-__device__ __forceinline__ void tc_load(unsigned addr, uint32_t (&r)[COLS]);
-template <>
-__device__ __forceinline__ void tc_load<32>(unsigned addr, uint32_t (&r)[32]) {
+// 32 columns of the warp's 32 lanes.  tc_loaded waits for all that is on its way; registers are handed through tc_use behind it, so that
+// nobody reads them earlier.
+__device__ __forceinline__ void tc_load32(unsigned addr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-                 "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(addr)
                  : "memory");
+}
+__device__ __forceinline__ void tc_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_use(uint32_t* r) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                      "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 // acc[2 i .. 2 i + 1] += s * (d0, d1)
 __device__ __forceinline__ void add_scaled(u64& acc, u64 s, uint32_t d0, uint32_t d1) {
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
     // A stage: hidden states [2 blocks][N][128 bytes], weights [2 blocks][8 pairs][1024].  Tensor memory, for each half of the rows 256
     // columns: two blocks of weights (32 columns each), then the sums of `slots` groups.
     constexpr int x_bytes = 2 * N * 128, kStage = stage_bytes<N>();
-    constexpr int slots = N <= 48 ? 4 : 2;
+    constexpr int slots = 192 / N < 4 ? 192 / N : 4;
     static_assert(slots * N <= 192, "tensor memory");
     const unsigned bars = smem_u32(&B.barriers[0]), stage0 = smem_u32(smem);
     const unsigned bars_end = bars + 8 * P.stages;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
     if (tid == 0) {
         for (int i = 0; i < P.stages; ++i) {
             barrier_init(bars + kFull + 8 * i, 1);
-            barrier_init(bars + kEmpty + 8 * i, 10);     // eight warps have their weights, two issuers their products
+            barrier_init(bars + kEmpty + 8 * i, 18);     // sixteen warps have their weights, two issuers their products
         }
         for (int g = 0; g < 2; ++g) {
             const unsigned h = bars + kHalf0 + g * kHalf;
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
         B.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before_sync();
@@ -142,13 +144,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
     __syncthreads();
     tc_after_sync();
     const unsigned tmem = B.tmem;
-    // The launch's 640 x 96 registers: 256 threads that add up, 256 that unpack, 128 others.
-    constexpr int kAdd = 144, kUnpack = 72, kOthers = 40;
-    static_assert(256 * kAdd + 256 * kUnpack + 128 * kOthers <= kManyThreads * 96, "a split of more registers than the launch has waits for ever");
+    // The launch's 896 x 72 registers: 256 threads that add up, 512 that unpack, 128 others.
+    constexpr int kAdd = 144, kUnpack = 48, kOthers = 24;
+    static_assert(256 * kAdd + 512 * kUnpack + 128 * kOthers <= kManyThreads * 72, "a split of more registers than the launch has waits for ever");
 
-    if (warp >= 16) {
+    if (warp >= 24) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOthers));
-        if (warp == 18) {
+        if (warp == 26) {
             // ------------------------------------------------------------------------------------ copies
             const int64_t unit_w = (int64_t)blocks * 8192;
             unsigned full = bars, st = stage0, phase = 1;    // (a fresh barrier's phase before the first has ended)
@@ -186,16 +188,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
                     int never = 0;
                     barrier_wait(full, phase ^ 1, &never);
                 }
-        } else if (warp < 18) {
+        } else if (warp < 26) {
             // ------------------------------------------------------------------------------------ products of half `wg`
-            const int wg = warp - 16;
+            const int wg = warp - 24;
             if (elect_one()) {
                 constexpr bool bf16 = std::is_same<X, __nv_bfloat16>::value;
                 constexpr unsigned what = 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (unsigned)(N >> 3) << 17 | (128u >> 4) << 24;
                 const unsigned a0 = tmem + wg * 256, d0 = a0 + 64, half_bars = bars + kHalf0 + wg * kHalf;
                 // K-major rows of 128 bytes, swizzled, eight rows every 1024 bytes
                 const u64 desc0 = 1ull << 16 | (u64)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61 | (u64)((stage0 & 0x3FFFF) >> 4);
-                unsigned full = bars, phase = 0, ab = 0, a_phase = 0, slot = 0, d_phase = 1;
+                unsigned full = bars, phase = 0, a_phase[2] = {0, 0}, slot = 0, d_phase = 1;
                 u64 stage = desc0;
                 for (int u = 0; u < mine && !*dead; ++u)
                     for (int c = 0; c < chunks; ++c) {
@@ -204,10 +206,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             if (2 * c + k >= blocks) break;
-                            barrier_wait(half_bars + kAFull + ab * 8, a_phase, dead);
+                            barrier_wait(half_bars + kAFull + k * 8, a_phase[k], dead);
+                            a_phase[k] ^= 1;
                             tc_after_sync();
                             const u64 desc = stage + (unsigned)(k * N * 8);
-                            const unsigned from = a0 + ab * 32;
+                            const unsigned from = a0 + k * 32;
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
                                 const bool begins = GS == 1 || (half == 0 && (GS == 2 || k == 0)), ends = GS == 1 || (half == 1 && (GS == 2 || k == 1));
@@ -219,13 +222,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
                                 tc_mma(d0 + slot * N, from + half * 16 + 8, desc + (half * 4 + 2), what, true);
                                 if (ends) {
                                     tc_commit(half_bars + kDFull + slot * 8);
-                                    slot = (slot + 1) & (slots - 1);
+                                    slot = slot + 1 == slots ? 0 : slot + 1;
                                     d_phase ^= slot == 0;
                                 }
                             }
-                            tc_commit(half_bars + kAEmpty + ab * 8);
-                            ab ^= 1;
-                            a_phase ^= ab == 0;
+                            tc_commit(half_bars + kAEmpty + k * 8);
                         }
                         tc_commit(full + kEmpty);
                         full += 8, stage += kStage / 16;
@@ -239,55 +240,47 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
             __syncwarp();
         }
     } else if (warp >= 8) {
-        // ---------------------------------------------------------------------------------------- unpacking
+        // ---------------------------------------------------------------------------------------- unpacking: block `k` of every chunk
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpack));
-        const int wg = (warp - 8) >> 2, wr = warp & 3;
-        const unsigned a0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256, half_bars = bars + kHalf0 + wg * kHalf;
+        const int k = (warp - 8) >> 3, wg = warp >> 2 & 1, wr = warp & 3;
+        const unsigned a0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + k * 32, half_bars = bars + kHalf0 + wg * kHalf + k * 8;
         const Unpack<X> unpack;
-        const unsigned own0 = stage0 + x_bytes + (wg * 4 + wr) * 1024 + lane * 16;
+        const unsigned own0 = stage0 + x_bytes + k * 8192 + (wg * 4 + wr) * 1024 + lane * 16;
         unsigned full = bars, own = own0, phase = 0, a_phase = 1;
-        // Blocks alternate between the two places; a unit of an odd number of them leaves `ab` where it is for the next.
-        unsigned ab = 0;
-        auto store = [&](const uint4 (&w)[2]) {
-            uint32_t p[2][16];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[r][(half * 4 + i) * 2] = unpack.value(half ? w[r].z : w[r].x, i);
-                        p[r][(half * 4 + i) * 2 + 1] = unpack.value(half ? w[r].w : w[r].y, i);
-                    }
-            barrier_wait(half_bars + kAEmpty + ab * 8, a_phase, dead);
-            __syncwarp();
-            tc_after_sync();
-            tc_store(a0 + ab * 32, p[0]);
-            tc_store(a0 + (16u << 16) + ab * 32, p[1]);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_before_sync();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(half_bars + kAFull + ab * 8);
-            ab ^= 1;
-            a_phase ^= ab == 0;
-        };
-        auto load = [&](uint4 (&w)[2], unsigned from) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[r].x), "=r"(w[r].y), "=r"(w[r].z), "=r"(w[r].w) : "r"(from + r * 512));
-        };
         for (int u = 0; u < mine; ++u) {
             for (int c = 0; c < chunks; ++c) {
+                const bool there = 2 * c + k < blocks;
                 barrier_wait(full, phase, dead);
                 __syncwarp();
-                uint4 w0[2], w1[2];
-                load(w0, own);
-                load(w1, own + 8192);       // (a block that is not there: not used)
-                const unsigned empty = full + kEmpty;
+                if (there) {
+                    uint4 w[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[r].x), "=r"(w[r].y), "=r"(w[r].z), "=r"(w[r].w) : "r"(own + r * 512));
+                    uint32_t p[2][16];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                p[r][(half * 4 + i) * 2] = unpack.value(half ? w[r].z : w[r].x, i);
+                                p[r][(half * 4 + i) * 2 + 1] = unpack.value(half ? w[r].w : w[r].y, i);
+                            }
+                    barrier_wait(half_bars + kAEmpty, a_phase, dead);
+                    __syncwarp();
+                    a_phase ^= 1;
+                    tc_after_sync();
+                    tc_store(a0, p[0]);
+                    tc_store(a0 + (16u << 16), p[1]);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_before_sync();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(half_bars + kAFull);
+                }
+                if (lane == 0) barrier_arrive(full + kEmpty);   // the stage's weights have been read
                 own += kStage, full += 8;
                 if (full == bars_end) full = bars, own = own0, phase ^= 1;
-                store(w0);
-                if (lane == 0) barrier_arrive(empty);   // the stage's weights have been read
-                if (2 * c + 1 < blocks) store(w1);
             }
             if (__any_sync(0xffffffffu, *dead)) break;
         }
@@ -316,6 +309,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) acc[i] = 0ull;
         unsigned slot = 0, d_phase = 0;
+        constexpr int kCols = N == 64 ? 64 : 32;     // taken out at a time
         fetch(blocks > 1);
         for (int u = 0; u < mine; ++u) {
             for (int c = 0; c < chunks; ++c) {
@@ -341,18 +335,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
                     u64 s2;
                     asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(scale[e]));
 #pragma unroll
-                    for (int c0 = 0; c0 < N; c0 += 32) {
-                        uint32_t v[32];
-                        tc_load<32>(d0 + slot * N + c0, v);
-                        if (c0 + 32 == N) {   // the columns may be written again
+                    for (int c0 = 0; c0 < N; c0 += kCols) {
+                        uint32_t v[kCols];
+#pragma unroll
+                        for (int i = 0; i < kCols; i += 32) tc_load32(d0 + slot * N + c0 + i, v + i);
+                        tc_loaded();
+#pragma unroll
+                        for (int i = 0; i < kCols; i += 16) tc_use(v + i);
+                        if (c0 + kCols == N) {   // the columns may be written again
                             tc_before_sync();
                             __syncwarp();
                             if (lane == 0) barrier_arrive(half_bars + kDEmpty + slot * 8);
                         }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) add_scaled(acc[c0 / 2 + i], s2, v[2 * i], v[2 * i + 1]);
+                        for (int i = 0; i < kCols / 2; ++i) add_scaled(acc[c0 / 2 + i], s2, v[2 * i], v[2 * i + 1]);
                     }
-                    slot = (slot + 1) & (slots - 1);
+                    slot = slot + 1 == slots ? 0 : slot + 1;
                     d_phase ^= slot == 0;
                 }
             }
@@ -373,7 +371,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
         tc_before_sync();
     }
     __syncthreads();
-    if (warp == 16) {
+    if (warp == 24) {
         tc_after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
