@@ -1,8 +1,8 @@
 // fsb_head_many.cu - the LM head (fsb_head.cu) for more hidden states than a warp's own tensor instructions are good for: tcgen05.mma with
 // the weights as operand A in tensor memory, unpacked there by the warps that later take the sums out again.
 //
-// A CTA takes 256 vocabulary rows at a time, in two halves, and all hidden states of the pass (up to 96).  Warps have one part each:
-// sixteen unpack weights (32 rows of every second block of 64 weights each) to q - 8 in bf16 / fp16, which is exact, and store them to tensor
+// A CTA takes 256 vocabulary rows at a time, in two halves, and all hidden states of the pass (up to 144).  Warps have one part each:
+// some unpack weights (32 rows of a block of 64 weights at a time) to q - 8 in bf16 / fp16, which is exact, and store them to tensor
 // memory as 32 columns of pairs; two issue the products of 128 rows; eight take the sums of one group of weights out again, a thread
 // for every row and a register for every hidden state, and add them up times the row's scale, two to an instruction; one has weights
 // and hidden states copied into a ring of stages of two blocks.
@@ -16,9 +16,17 @@
 namespace fsb {
 namespace {
 
-constexpr int kManyThreads = 896;        // warps 0 - 7 take sums out, 8 - 23 unpack, 24 and 25 issue, 26 copies, 27 completes their group of four
+// Warps 0 - 7 take sums out, the next ones unpack, then two issue, one copies and one completes their group of four.  Registers of those
+// three kinds: a register per hidden state is what the first kind has; with more than 96 of them there is room for four warps that
+// unpack, which then is a matter of tensor instructions anyway.
+template <int N>
+struct Roles {
+    static constexpr int unpacking = N <= 96 ? 16 : 4, threads = 32 * (8 + unpacking + 4), launch_regs = N <= 96 ? 72 : 128;
+    static constexpr int add_regs = N <= 96 ? 144 : 192, unpack_regs = N <= 96 ? 48 : 88, other_regs = N <= 96 ? 24 : 40;
+    static_assert(256 * add_regs + 32 * unpacking * unpack_regs + 128 * other_regs <= threads * launch_regs, "a split of more registers than the launch has waits for ever");
+};
 constexpr int kRows = 256;               // vocabulary rows of a unit
-constexpr int kTokensMax = 96;
+constexpr int kTokensMax = 144;
 constexpr int kSharedMax = 227 * 1024;
 constexpr int kStagesMax = 8;
 
@@ -77,7 +85,7 @@ __device__ __forceinline__ void tc_store(unsigned addr, const uint32_t (&r)[16])
                  "r"(r[15])
                  : "memory");
 }
-// 32 columns of the warp's 32 lanes.  tc_loaded waits for all that is on its way; registers are handed through tc_use behind it, so that
+// 32 or 16 columns of the warp's 32 lanes.  tc_loaded waits for all that is on its way; registers are handed through tc_use behind it, so that
 // nobody reads them earlier.
 __device__ __forceinline__ void tc_load32(unsigned addr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
@@ -85,6 +93,13 @@ __device__ __forceinline__ void tc_load32(unsigned addr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
                    "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_load16(unsigned addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr)
                  : "memory");
 }
@@ -101,9 +116,9 @@ __device__ __forceinline__ void add_scaled(u64& acc, u64 s, uint32_t d0, uint32_
 template <int N>
 __host__ __device__ constexpr int stage_bytes() { return 2 * N * 128 + 16384; }
 
-// N: hidden states of a pass, rounded up to 32.
+// N: hidden states of a pass, rounded up to 32, 64, 96 or 144.
 template <class X, int GS, int N>
-__global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid_constant__ ManyPlan P, const __grid_constant__ CUtensorMap hidden_map) {
+__global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const __grid_constant__ ManyPlan P, const __grid_constant__ CUtensorMap hidden_map) {
     extern __shared__ __align__(1024) unsigned char smem_any[];
     __shared__ Control B;
     unsigned char* smem = smem_any + (-smem_u32(smem_any) & 1023u);   // (swizzled rows want 1024-byte boundaries)
@@ -125,7 +140,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
     if (tid == 0) {
         for (int i = 0; i < P.stages; ++i) {
             barrier_init(bars + kFull + 8 * i, 1);
-            barrier_init(bars + kEmpty + 8 * i, 18);     // sixteen warps have their weights, two issuers their products
+            barrier_init(bars + kEmpty + 8 * i, Roles<N>::unpacking + 2);     // weights have been read, products are done
         }
         for (int g = 0; g < 2; ++g) {
             const unsigned h = bars + kHalf0 + g * kHalf;
@@ -136,7 +151,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
         B.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 24) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before_sync();
@@ -144,13 +159,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
     __syncthreads();
     tc_after_sync();
     const unsigned tmem = B.tmem;
-    // The launch's 896 x 72 registers: 256 threads that add up, 512 that unpack, 128 others.
-    constexpr int kAdd = 144, kUnpack = 48, kOthers = 24;
-    static_assert(256 * kAdd + 512 * kUnpack + 128 * kOthers <= kManyThreads * 72, "a split of more registers than the launch has waits for ever");
-
-    if (warp >= 24) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOthers));
-        if (warp == 26) {
+    constexpr int others = 8 + Roles<N>::unpacking;
+    if (warp >= others) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles<N>::other_regs));
+        if (warp == others + 2) {
             // ------------------------------------------------------------------------------------ copies
             const int64_t unit_w = (int64_t)blocks * 8192;
             unsigned full = bars, st = stage0, phase = 1;    // (a fresh barrier's phase before the first has ended)
@@ -188,9 +200,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
                     int never = 0;
                     barrier_wait(full, phase ^ 1, &never);
                 }
-        } else if (warp < 26) {
+        } else if (warp < others + 2) {
             // ------------------------------------------------------------------------------------ products of half `wg`
-            const int wg = warp - 24;
+            const int wg = warp - others;
             if (elect_one()) {
                 constexpr bool bf16 = std::is_same<X, __nv_bfloat16>::value;
                 constexpr unsigned what = 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (unsigned)(N >> 3) << 17 | (128u >> 4) << 24;
@@ -240,23 +252,29 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
             __syncwarp();
         }
     } else if (warp >= 8) {
-        // ---------------------------------------------------------------------------------------- unpacking: block `k` of every chunk
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpack));
-        const int k = (warp - 8) >> 3, wg = warp >> 2 & 1, wr = warp & 3;
-        const unsigned a0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + k * 32, half_bars = bars + kHalf0 + wg * kHalf + k * 8;
+        // ---------------------------------------------------------------------------------------- unpacking
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles<N>::unpack_regs));
+        // A chunk has four parts, two blocks of two halves; four groups of warps have one each, one group has all.
+        constexpr int kParts = 16 / Roles<N>::unpacking;
+        const int wr = warp & 3, part0 = kParts == 1 ? (warp - 8) >> 2 : 0;
         const Unpack<X> unpack;
-        const unsigned own0 = stage0 + x_bytes + k * 8192 + (wg * 4 + wr) * 1024 + lane * 16;
-        unsigned full = bars, own = own0, phase = 0, a_phase = 1;
+        const unsigned own0 = stage0 + x_bytes + wr * 1024 + lane * 16;
+        unsigned full = bars, own = own0, phase = 0, a_phase[2] = {1, 1};
         for (int u = 0; u < mine; ++u) {
             for (int c = 0; c < chunks; ++c) {
-                const bool there = 2 * c + k < blocks;
                 barrier_wait(full, phase, dead);
                 __syncwarp();
-                if (there) {
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    const int k = (part0 + q) >> 1, wg = (part0 + q) & 1;
+                    if (2 * c + k >= blocks) break;
+                    const unsigned a0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + k * 32, half_bars = bars + kHalf0 + wg * kHalf + k * 8;
                     uint4 w[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[r].x), "=r"(w[r].y), "=r"(w[r].z), "=r"(w[r].w) : "r"(own + r * 512));
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[r].x), "=r"(w[r].y), "=r"(w[r].z), "=r"(w[r].w)
+                                     : "r"(own + k * 8192 + wg * 4096 + r * 512));
                     uint32_t p[2][16];
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
@@ -267,9 +285,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
                                 p[r][(half * 4 + i) * 2] = unpack.value(half ? w[r].z : w[r].x, i);
                                 p[r][(half * 4 + i) * 2 + 1] = unpack.value(half ? w[r].w : w[r].y, i);
                             }
-                    barrier_wait(half_bars + kAEmpty, a_phase, dead);
+                    const int which = kParts == 1 ? 0 : q >> 1;
+                    barrier_wait(half_bars + kAEmpty, a_phase[which], dead);
                     __syncwarp();
-                    a_phase ^= 1;
+                    if (kParts == 1 || wg == 1) a_phase[which] ^= 1;
                     tc_after_sync();
                     tc_store(a0, p[0]);
                     tc_store(a0 + (16u << 16), p[1]);
@@ -286,7 +305,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
         }
     } else {
         // ---------------------------------------------------------------------------------------- a thread for every row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAdd));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles<N>::add_regs));
         const int wg = warp >> 2, wr = warp & 3, r16 = lane >> 4, in16 = lane & 15;
         const unsigned d0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + 64, half_bars = bars + kHalf0 + wg * kHalf;
         const bool bf16_scales = a.scale_type == FSB_BF16;
@@ -337,18 +356,26 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
 #pragma unroll
                     for (int c0 = 0; c0 < N; c0 += kCols) {
                         uint32_t v[kCols];
+                        const unsigned from = d0 + slot * N + c0;
+                        constexpr int kLast = N % kCols ? N % kCols : kCols;     // columns of the last turn (16 or 32)
+                        const bool last = c0 + kCols >= N;
+                        if (last && kLast == 16) tc_load16(from, v);
+                        else {
 #pragma unroll
-                        for (int i = 0; i < kCols; i += 32) tc_load32(d0 + slot * N + c0 + i, v + i);
+                            for (int i = 0; i < kCols; i += 32) tc_load32(from + i, v + i);
+                        }
                         tc_loaded();
 #pragma unroll
-                        for (int i = 0; i < kCols; i += 16) tc_use(v + i);
-                        if (c0 + kCols == N) {   // the columns may be written again
+                        for (int i = 0; i < kCols; i += 16)
+                            if (c0 + i < N) tc_use(v + i);
+                        if (last) {   // the columns may be written again
                             tc_before_sync();
                             __syncwarp();
                             if (lane == 0) barrier_arrive(half_bars + kDEmpty + slot * 8);
                         }
 #pragma unroll
-                        for (int i = 0; i < kCols / 2; ++i) add_scaled(acc[c0 / 2 + i], s2, v[2 * i], v[2 * i + 1]);
+                        for (int i = 0; i < kCols / 2; ++i)
+                            if (c0 + 2 * i < N) add_scaled(acc[c0 / 2 + i < N / 2 ? c0 / 2 + i : 0], s2, v[2 * i], v[2 * i + 1]);
                     }
                     slot = slot + 1 == slots ? 0 : slot + 1;
                     d_phase ^= slot == 0;
@@ -371,7 +398,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) head_many_kernel(const __grid
         tc_before_sync();
     }
     __syncthreads();
-    if (warp == 24) {
+    if (warp == 8) {
         tc_after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
@@ -401,12 +428,13 @@ int run(ManyPlan p, const CUtensorMap& map, cudaStream_t stream) {
     const int units = (p.a.n_vocab + kRows - 1) / kRows;
     const dim3 grid((unsigned)std::min(units, p.a.sms), (unsigned)((p.a.n_rows + p.tokens - 1) / p.tokens));
     p.stages = std::min(kStagesMax, (kSharedMax - 3072) / stage_bytes<N>());
-    head_many_kernel<X, GS, N><<<grid, kManyThreads, (size_t)(p.stages * stage_bytes<N>() + 1024), stream>>>(p, map);
+    head_many_kernel<X, GS, N><<<grid, Roles<N>::threads, (size_t)(p.stages * stage_bytes<N>() + 1024), stream>>>(p, map);
     return (int)cudaGetLastError();
 }
 template <class X, int GS>
 int run_columns(const ManyPlan& p, const CUtensorMap& map, cudaStream_t stream) {
-    return p.tokens <= 32 ? run<X, GS, 32>(p, map, stream) : p.tokens <= 64 ? run<X, GS, 64>(p, map, stream) : run<X, GS, 96>(p, map, stream);
+    return p.tokens <= 32 ? run<X, GS, 32>(p, map, stream) : p.tokens <= 64 ? run<X, GS, 64>(p, map, stream)
+           : p.tokens <= 96 ? run<X, GS, 96>(p, map, stream) : run<X, GS, 144>(p, map, stream);
 }
 template <class X>
 int run_group(const ManyPlan& p, const CUtensorMap& map, cudaStream_t stream) {
@@ -418,6 +446,7 @@ int prepare_columns() {
     cudaError_t e = cudaFuncSetAttribute(head_many_kernel<X, GS, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, 96>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, 144>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
     return (int)e;
 }
 template <class X>
@@ -445,7 +474,7 @@ bool launch_head_many(const HeadArgs& a, void* stream, int* error) {
     p.tokens = (a.n_rows + passes - 1) / passes;
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)a.n_hidden, (cuuint64_t)a.n_rows}, strides[1] = {(cuuint64_t)a.ld_hidden * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)((p.tokens + 31) / 32 * 32)}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {64, (cuuint32_t)(p.tokens <= 96 ? (p.tokens + 31) / 32 * 32 : 144)}, step[2] = {1, 1};
     if (encode(&map, a.hidden_type == FSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.hidden), dims, strides, box, step,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
