@@ -133,6 +133,8 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_kernel(const __grid_consta
     constexpr int kVecs = kCols / VEC;
     constexpr unsigned kAll = (1u << VEC) - 1u, kEvery = (1u << kCols) - 1u;
     extern __shared__ __align__(16) unsigned char smem[];
+    pdl_launch_dependents();
+    pdl_wait_prior();
     const AdjustArgs& a = P.a;
     const int row = (int)blockIdx.y, tid = (int)threadIdx.x;
     const AdjustRow& R = P.rows[row];
@@ -329,8 +331,7 @@ int launch_rows(const AdjustArgs& a, const AdjustRow* rows, int n_rows, cudaStre
     }
     p.tile = batches * kBatch;
     const dim3 grid((unsigned)((a.n_vocab + p.tile - 1) / p.tile), (unsigned)n_rows);
-    adjust_kernel<TI, TO, VEC, ROWS, WIDE><<<grid, kThreads, (size_t)Special<WIDE>::bytes(p.tile), stream>>>(p);
-    return (int)cudaGetLastError();
+    return launch_chained(adjust_kernel<TI, TO, VEC, ROWS, WIDE>, grid, kThreads, (size_t)Special<WIDE>::bytes(p.tile), stream, a.chained != 0, p);
 }
 
 template <class TI, class TO, int VEC>

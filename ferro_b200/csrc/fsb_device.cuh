@@ -92,6 +92,23 @@ __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)_
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Launches with programmatic stream serialization if `chained`: the kernel's CTAs are placed while the launch before it ends, and the
+// kernel has to call pdl_wait_prior before it touches memory.
+template <class... K, class... A>
+int launch_chained(void (*kernel)(K...), dim3 grid, int threads, size_t shared, cudaStream_t stream, bool chained, const A&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = chained ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Thread-block clusters (the CTAs that share a row): the address of a shared-memory location in another CTA of the
 // cluster, stores to it, and the cluster's barrier (arrive releases this thread's stores to the cluster, wait acquires
 // the others').

@@ -21,9 +21,15 @@ namespace {
 #ifndef HEAD_FEW
 #define HEAD_FEW 16
 #endif
-constexpr int kWarps = 16;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kAhead = 4;                    // blocks of 64 weights that a warp has on their way
+#ifndef HEAD_W1
+#define HEAD_W1 28
+#define HEAD_A1 2
+#endif
+// Warps of a CTA, and blocks of 64 weights that each has on their way.
+template <int NT>
+struct Shape {
+    static constexpr int warps = NT == 1 ? HEAD_W1 : 16, ahead = NT == 1 ? HEAD_A1 : 4;
+};
 constexpr int kSharedMax = 227 * 1024;
 
 // ------------------------------------------------------------------------------------------------ layout
@@ -102,7 +108,8 @@ __device__ __forceinline__ float sum_of(uint32_t pair) {
 // registers: the weights go from memory to the tensor cores without touching shared memory.  The warps that share a unit add up
 // their parts in shared memory, in a fixed order.
 template <class X, int GS, int NT>
-__global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant__ HeadPlan P) {
+__global__ void __launch_bounds__(32 * Shape<NT>::warps, 1) head_kernel(const __grid_constant__ HeadPlan P) {
+    constexpr int kWarps = Shape<NT>::warps, kThreads = 32 * kWarps, kAhead = Shape<NT>::ahead;
     extern __shared__ __align__(16) unsigned char smem[];
     const HeadArgs& a = P.a;
     constexpr int kBuffers = 2;
@@ -138,6 +145,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
             else sc[i][r].x = __ldg(reinterpret_cast<const unsigned*>(q + r * 32));
         }
     };
+    pdl_launch_dependents();
+    pdl_wait_prior();
     if (first < pairs) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
@@ -285,15 +294,14 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
 
 int shared_bytes(const HeadArgs& a, int nt, int tokens) {
     const int blocks = row_blocks(a.n_hidden), groups = (2 * blocks * 32 + a.group - 1) / a.group;
-    return 4 * (2 * kWarps * nt * 8 * 36 + groups * nt * 8) + blocks * 128 * tokens;
+    return 4 * (2 * (nt == 1 ? Shape<1>::warps : Shape<2>::warps) * nt * 8 * 36 + groups * nt * 8) + blocks * 128 * tokens;
 }
 
 template <class X, int GS, int NT>
 int launch_plan(const HeadPlan& p, int grid_x, cudaStream_t stream) {
     const int bytes = shared_bytes(p.a, NT, p.tokens);
     const dim3 grid((unsigned)grid_x, (unsigned)((p.a.n_rows + p.tokens - 1) / p.tokens));
-    head_kernel<X, GS, NT><<<grid, kThreads, (size_t)bytes, stream>>>(p);
-    return (int)cudaGetLastError();
+    return launch_chained(head_kernel<X, GS, NT>, grid, 32 * Shape<NT>::warps, (size_t)bytes, stream, p.a.chained != 0, p);
 }
 template <class X, int GS>
 int launch_tokens(const HeadPlan& p, int nt, int grid_x, cudaStream_t stream) {
@@ -360,9 +368,11 @@ int launch_head(const HeadArgs& a, void* stream, int* launches) {
     const int pairs = (a.n_vocab + 31) / 32, pieces = row_blocks(a.n_hidden) / (a.group == 128 ? 2 : 1);
     int64_t best = 0;
     int grid_x = 1;
-    for (int ks = 1; ks <= kWarps; ks *= 2) {
+    const int warps = nt == 1 ? Shape<1>::warps : Shape<2>::warps;
+    for (int ks = 1; ks <= warps; ++ks) {
         if (ks > pieces) break;
-        const int per_cta = kWarps / ks, ctas = std::min(a.sms, (pairs + per_cta - 1) / per_cta);
+        if (warps % ks) continue;
+        const int per_cta = warps / ks, ctas = std::min(a.sms, (pairs + per_cta - 1) / per_cta);
         const int64_t waves = ((int64_t)pairs + (int64_t)ctas * per_cta - 1) / ((int64_t)ctas * per_cta), longest = (pieces + ks - 1) / ks;
         const int64_t cost = waves * (longest * 16 + 8 + ks);   // (a share's end costs about half a step, and more for every part that is added)
         if (best == 0 || cost < best) {

@@ -158,6 +158,8 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
     }
     __syncthreads();
     tc_after_sync();
+    pdl_launch_dependents();
+    pdl_wait_prior();
     const unsigned tmem = B.tmem;
     constexpr int others = 8 + Roles<N>::unpacking;
     if (warp >= others) {
@@ -428,8 +430,7 @@ int run(ManyPlan p, const CUtensorMap& map, cudaStream_t stream) {
     const int units = (p.a.n_vocab + kRows - 1) / kRows;
     const dim3 grid((unsigned)std::min(units, p.a.sms), (unsigned)((p.a.n_rows + p.tokens - 1) / p.tokens));
     p.stages = std::min(kStagesMax, (kSharedMax - 3072) / stage_bytes<N>());
-    head_many_kernel<X, GS, N><<<grid, Roles<N>::threads, (size_t)(p.stages * stage_bytes<N>() + 1024), stream>>>(p, map);
-    return (int)cudaGetLastError();
+    return launch_chained(head_many_kernel<X, GS, N>, grid, Roles<N>::threads, (size_t)(p.stages * stage_bytes<N>() + 1024), stream, p.a.chained != 0, p, map);
 }
 template <class X, int GS>
 int run_columns(const ManyPlan& p, const CUtensorMap& map, cudaStream_t stream) {

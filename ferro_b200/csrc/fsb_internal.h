@@ -159,6 +159,7 @@ struct AdjustArgs {
     int32_t first_row;         // the call's number of row 0
     int32_t vocab_offset;      // token id of column 0
     float softcap;             // 0 = off
+    int32_t chained;           // placed while the launch before it in the stream ends (not in a stream that is being captured)
 };
 // Launches for n_rows rows; rows_host is read before the call returns.  Returns a cudaError_t as int.
 int launch_adjust(const AdjustArgs& a, const AdjustRow* rows_host, void* stream, int* launches);
@@ -177,6 +178,7 @@ struct HeadArgs {
     int32_t n_rows, n_vocab, n_hidden, group;
     int32_t scale_type, hidden_type;
     int32_t sms;
+    int32_t chained;           // as in AdjustArgs
     uint32_t* late;            // a pinned host word that is set if a wait inside the kernel ran out
 };
 int prepare_head_kernels();   // for the current device, before its first launch_head

@@ -114,6 +114,7 @@ int queue_adjust(fsb_handle* h, int n_rows, const int* stream_ids, const void* l
     a.n_vocab = n_vocab;
     a.vocab_offset = h->vocab_offset;
     a.softcap = h->softcap;
+    a.chained = 1;
     if (report_empty) *static_cast<volatile uint32_t*>(h->h_empty) = 0u;
     int launches = 0;
     const int e = launch_adjust(a, rows.data(), h->stream, &launches);
@@ -255,6 +256,7 @@ int queue_head(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidd
     a.hidden_type = hidden_type;
     a.sms = h->sm_count;
     a.late = h->h_empty_dev + 1;
+    a.chained = is_capturing(h) ? 0 : 1;
     int launches = 0;
     const int e = launch_head(a, h->stream, &launches);
     h->counters.kernel_launches += (uint64_t)launches;
