@@ -18,17 +18,12 @@
 namespace fsb {
 namespace {
 
-#ifndef HEAD_FEW
-#define HEAD_FEW 16
-#endif
-#ifndef HEAD_W1
-#define HEAD_W1 28
-#define HEAD_A1 2
-#endif
-// Warps of a CTA, and blocks of 64 weights that each has on their way.
-template <int NT>
+// Warps of a CTA, and blocks of 64 weights that each has on their way.  28 warps of 72 registers are the faster shape for up to eight hidden
+// states (1 x 262144 x 2560, groups of 128: 67.7 us, 69.9 with 16 of 128; 8 x 65536 x 2048 22.8, 24.8), but what they share out has to come
+// out even (5 x 100003 x 2016: 38.9, 35.0): launch_head counts.
+template <int WARPS>
 struct Shape {
-    static constexpr int warps = NT == 1 ? HEAD_W1 : 16, ahead = NT == 1 ? HEAD_A1 : 4;
+    static constexpr int ahead = WARPS == 16 ? 4 : 2;
 };
 constexpr int kSharedMax = 227 * 1024;
 
@@ -70,6 +65,8 @@ struct HeadPlan {
     HeadArgs a;
     int ksplit;        // warps that share a tile pair's k; the CTA's other warps take other tile pairs
     int tokens;        // hidden states a pass
+    int eights;        // ... rounded up to eight
+    int warps, ctas;
     int vec;           // hidden states may be read 16 bytes at a time
 };
 
@@ -107,9 +104,9 @@ __device__ __forceinline__ float sum_of(uint32_t pair) {
 // A warp works through units of 32 vocabulary rows and its share of their k, block by block, with kAhead blocks on their way in
 // registers: the weights go from memory to the tensor cores without touching shared memory.  The warps that share a unit add up
 // their parts in shared memory, in a fixed order.
-template <class X, int GS, int NT>
-__global__ void __launch_bounds__(32 * Shape<NT>::warps, 1) head_kernel(const __grid_constant__ HeadPlan P) {
-    constexpr int kWarps = Shape<NT>::warps, kThreads = 32 * kWarps, kAhead = Shape<NT>::ahead;
+template <class X, int GS, int NT, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, 1) head_kernel(const __grid_constant__ HeadPlan P) {
+    constexpr int kThreads = 32 * kWarps, kAhead = Shape<kWarps>::ahead;
     extern __shared__ __align__(16) unsigned char smem[];
     const HeadArgs& a = P.a;
     constexpr int kBuffers = 2;
@@ -146,12 +143,13 @@ __global__ void __launch_bounds__(32 * Shape<NT>::warps, 1) head_kernel(const __
         }
     };
     pdl_launch_dependents();
-    pdl_wait_prior();
-    if (first < pairs) {
+    if (first < pairs) {   // (no launch in the stream writes weights)
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
             if (i < steps) fetch(i, first, i);
     }
+
+    pdl_wait_prior();
 
     // Hidden states into shared memory: per half and lane t the pairs 8 i + 2 t, 16 bytes.  Odd states have their halves swapped, so
     // that the lanes of a quarter warp read 128 different bytes of 128.
@@ -292,31 +290,30 @@ __global__ void __launch_bounds__(32 * Shape<NT>::warps, 1) head_kernel(const __
     }
 }
 
-int shared_bytes(const HeadArgs& a, int nt, int tokens) {
+int shared_bytes(const HeadArgs& a, int nt, int warps, int tokens) {
     const int blocks = row_blocks(a.n_hidden), groups = (2 * blocks * 32 + a.group - 1) / a.group;
-    return 4 * (2 * (nt == 1 ? Shape<1>::warps : Shape<2>::warps) * nt * 8 * 36 + groups * nt * 8) + blocks * 128 * tokens;
+    return 4 * (2 * warps * nt * 8 * 36 + groups * nt * 8) + blocks * 128 * tokens;
 }
 
-template <class X, int GS, int NT>
-int launch_plan(const HeadPlan& p, int grid_x, cudaStream_t stream) {
-    const int bytes = shared_bytes(p.a, NT, p.tokens);
-    const dim3 grid((unsigned)grid_x, (unsigned)((p.a.n_rows + p.tokens - 1) / p.tokens));
-    return launch_chained(head_kernel<X, GS, NT>, grid, 32 * Shape<NT>::warps, (size_t)bytes, stream, p.a.chained != 0, p);
+template <class X, int GS, int NT, int WARPS>
+int launch_plan(const HeadPlan& p, cudaStream_t stream) {
+    const dim3 grid((unsigned)p.ctas, (unsigned)((p.a.n_rows + p.tokens - 1) / p.tokens));
+    return launch_chained(head_kernel<X, GS, NT, WARPS>, grid, 32 * WARPS, (size_t)shared_bytes(p.a, NT, WARPS, p.tokens), stream, p.a.chained != 0, p);
 }
 template <class X, int GS>
-int launch_tokens(const HeadPlan& p, int nt, int grid_x, cudaStream_t stream) {
-    return nt == 1 ? launch_plan<X, GS, 1>(p, grid_x, stream) : launch_plan<X, GS, 2>(p, grid_x, stream);
+int launch_shape(const HeadPlan& p, cudaStream_t stream) {
+    return p.eights == 2 ? launch_plan<X, GS, 2, 16>(p, stream) : p.warps == 16 ? launch_plan<X, GS, 1, 16>(p, stream) : launch_plan<X, GS, 1, 28>(p, stream);
 }
 template <class X>
-int launch_group(const HeadPlan& p, int nt, int grid_x, cudaStream_t stream) {
-    return p.a.group == 32 ? launch_tokens<X, 1>(p, nt, grid_x, stream)
-           : p.a.group == 64 ? launch_tokens<X, 2>(p, nt, grid_x, stream) : launch_tokens<X, 4>(p, nt, grid_x, stream);
+int launch_group(const HeadPlan& p, cudaStream_t stream) {
+    return p.a.group == 32 ? launch_shape<X, 1>(p, stream) : p.a.group == 64 ? launch_shape<X, 2>(p, stream) : launch_shape<X, 4>(p, stream);
 }
 
 template <class X, int GS>
 int prepare_group() {
-    cudaError_t e = cudaFuncSetAttribute(head_kernel<X, GS, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_kernel<X, GS, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax);
+    cudaError_t e = cudaFuncSetAttribute(head_kernel<X, GS, 1, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_kernel<X, GS, 1, 28>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_kernel<X, GS, 2, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax);
     return (int)e;
 }
 template <class X>
@@ -352,36 +349,41 @@ int launch_head(const HeadArgs& a, void* stream, int* launches) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ++*launches;
     int error = 0;
-    if (a.n_rows > HEAD_FEW && launch_head_many(a, stream, &error)) return error;
+    // More hidden states than eight (groups of 32: than sixteen, since every group's sums have to be taken out of tensor memory) are the
+    // other kernel's.  us here and there, 16 x 65536 x 1024 (32) 18.2, 19.2; 16 x 262144 x 2560 (32) 121, 133, (128) 98, 87; 9 of them
+    // (32) 113, 132, (128) 92, 85; 9 x 65536 x 2048 (64) 25.9, 26.0; eight of them run here in 19.8 (32).
+    if (a.n_rows > (a.group == 32 ? 16 : 8) && launch_head_many(a, stream, &error)) return error;
     HeadPlan p{};
     p.a = a;
     p.vec = reinterpret_cast<uintptr_t>(a.hidden) % 16 == 0 && a.ld_hidden % 8 == 0;
-    // as many hidden states a pass as shared memory holds beside the partial sums, up to 16
-    int nt = a.n_rows > 8 ? 2 : 1;
-    p.tokens = std::min(8 * nt, a.n_rows);
-    if (shared_bytes(a, nt, p.tokens) > kSharedMax) {
-        nt = 1;
-        p.tokens = std::min(8, a.n_rows);
-        while (shared_bytes(a, 1, p.tokens) > kSharedMax) --p.tokens;
-    }
-    // How many warps share the k of 32 rows: the fewest steps of the CTA with the most, its waves times the longest share.
+    // How a launch is laid out: warps of a CTA, and how many of them share the k of 32 vocabulary rows.  The fewest steps of the CTA with the
+    // most, its waves times the longest share (a share's end costs about half a step, and more for every part that is added), counted in
+    // the time of all warps; the 28 take 0.95 of the time of the 16.
     const int pairs = (a.n_vocab + 31) / 32, pieces = row_blocks(a.n_hidden) / (a.group == 128 ? 2 : 1);
-    int64_t best = 0;
-    int grid_x = 1;
-    const int warps = nt == 1 ? Shape<1>::warps : Shape<2>::warps;
-    for (int ks = 1; ks <= warps; ++ks) {
-        if (ks > pieces) break;
-        if (warps % ks) continue;
-        const int per_cta = warps / ks, ctas = std::min(a.sms, (pairs + per_cta - 1) / per_cta);
-        const int64_t waves = ((int64_t)pairs + (int64_t)ctas * per_cta - 1) / ((int64_t)ctas * per_cta), longest = (pieces + ks - 1) / ks;
-        const int64_t cost = waves * (longest * 16 + 8 + ks);   // (a share's end costs about half a step, and more for every part that is added)
-        if (best == 0 || cost < best) {
-            best = cost;
-            p.ksplit = ks;
-            grid_x = ctas;
+    double best = 0.0;
+    for (const int warps : {16, 28}) {
+        const int eights = warps == 16 && a.n_rows > 8 ? 2 : 1;
+        if (warps == 28 && a.n_rows > 8) continue;
+        // as many hidden states a pass as shared memory holds beside the partial sums
+        int tokens = std::min(8 * eights, a.n_rows);
+        while (tokens > 1 && shared_bytes(a, eights, warps, tokens) > kSharedMax) --tokens;
+        const int passes = (a.n_rows + tokens - 1) / tokens;
+        for (int ks = 1; ks <= std::min(warps, pieces); ++ks) {
+            if (warps % ks) continue;
+            const int per_cta = warps / ks, ctas = std::min(a.sms, (pairs + per_cta - 1) / per_cta);
+            const int64_t waves = ((int64_t)pairs + (int64_t)ctas * per_cta - 1) / ((int64_t)ctas * per_cta), longest = (pieces + ks - 1) / ks;
+            const double cost = (double)passes * (double)waves * (16.0 * (double)longest + 8.0 + ks) * (warps == 28 ? 28 * 0.95 : 16.0);
+            if (best == 0.0 || cost < best) {
+                best = cost;
+                p.warps = warps;
+                p.eights = eights;
+                p.tokens = tokens;
+                p.ksplit = ks;
+                p.ctas = ctas;
+            }
         }
     }
-    return a.hidden_type == FSB_BF16 ? launch_group<__nv_bfloat16>(p, nt, grid_x, s) : launch_group<__half>(p, nt, grid_x, s);
+    return a.hidden_type == FSB_BF16 ? launch_group<__nv_bfloat16>(p, s) : launch_group<__half>(p, s);
 }
 
 }  // namespace fsb

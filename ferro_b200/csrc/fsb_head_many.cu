@@ -16,15 +16,22 @@
 namespace fsb {
 namespace {
 
-// Warps 0 - 7 take sums out, the next ones unpack, then two issue, one copies and one completes their group of four.  Registers of those
-// three kinds: a register per hidden state is what the first kind has; with more than 96 of them there is room for four warps that
-// unpack, which then is a matter of tensor instructions anyway.
-template <int N>
-struct Roles {
-    static constexpr int unpacking = N <= 96 ? 16 : 4, threads = 32 * (8 + unpacking + 4), launch_regs = N <= 96 ? 72 : 128;
-    static constexpr int add_regs = N <= 96 ? 144 : 192, unpack_regs = N <= 96 ? 48 : 88, other_regs = N <= 96 ? 24 : 40;
-    static_assert(256 * add_regs + 32 * unpacking * unpack_regs + 128 * other_regs <= threads * launch_regs, "a split of more registers than the launch has waits for ever");
+// How many warps take sums out (the first ones), how many unpack (the next ones; then two issue, one copies and one completes their group
+// of four), and the registers of the three kinds: a register per hidden state is what the first kind has.
+template <int ADD, int UNPACK, int LAUNCH_REGS, int ADD_REGS, int UNPACK_REGS, int OTHER_REGS>
+struct Split {
+    static constexpr int adding = ADD, unpacking = UNPACK, threads = 32 * (ADD + UNPACK + 4), add_regs = ADD_REGS, unpack_regs = UNPACK_REGS, other_regs = OTHER_REGS;
+    static_assert(32 * ADD * ADD_REGS + 32 * UNPACK * UNPACK_REGS + 128 * OTHER_REGS <= threads * LAUNCH_REGS, "a split of more registers than the launch has waits for ever");
 };
+// For 64 and 96 hidden states eight warps take out as much as sixteen with half of the columns each, in fewer instructions (64 and 96 x
+// 262144 x 2560, groups of 32: 177 and 214 us; 184 and 324); for 32 the latency of taking out counts (135; 121).  For 144 there are
+// registers for four warps that unpack, which is then a matter of tensor instructions anyway.
+template <int N>
+struct Roles : Split<8, 16, 72, 144, 48, 24> {};
+template <>
+struct Roles<32> : Split<16, 8, 72, 88, 56, 32> {};
+template <>
+struct Roles<144> : Split<8, 4, 128, 192, 88, 40> {};
 constexpr int kRows = 256;               // vocabulary rows of a unit
 constexpr int kTokensMax = 144;
 constexpr int kSharedMax = 227 * 1024;
@@ -135,6 +142,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
     static_assert(slots * N <= 192, "tensor memory");
     const unsigned bars = smem_u32(&B.barriers[0]), stage0 = smem_u32(smem);
     const unsigned bars_end = bars + 8 * P.stages;
+    constexpr int adding = Roles<N>::adding, others = adding + Roles<N>::unpacking;
     volatile int* dead = &B.dead;
 
     if (tid == 0) {
@@ -145,13 +153,13 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
         for (int g = 0; g < 2; ++g) {
             const unsigned h = bars + kHalf0 + g * kHalf;
             for (int i = 0; i < 2; ++i) barrier_init(h + kAFull + 8 * i, 4), barrier_init(h + kAEmpty + 8 * i, 1);
-            for (int i = 0; i < 4; ++i) barrier_init(h + kDFull + 8 * i, 1), barrier_init(h + kDEmpty + 8 * i, 4);
+            for (int i = 0; i < 4; ++i) barrier_init(h + kDFull + 8 * i, 1), barrier_init(h + kDEmpty + 8 * i, Roles<N>::adding / 2);
             barrier_init(h + kDone, 1);
         }
         B.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == others) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&B.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before_sync();
@@ -161,7 +169,6 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
     pdl_launch_dependents();
     pdl_wait_prior();
     const unsigned tmem = B.tmem;
-    constexpr int others = 8 + Roles<N>::unpacking;
     if (warp >= others) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles<N>::other_regs));
         if (warp == others + 2) {
@@ -253,12 +260,12 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
             }
             __syncwarp();
         }
-    } else if (warp >= 8) {
+    } else if (warp >= adding) {
         // ---------------------------------------------------------------------------------------- unpacking
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles<N>::unpack_regs));
-        // A chunk has four parts, two blocks of two halves; four groups of warps have one each, one group has all.
+        // A chunk has four parts, two blocks of two halves, shared out evenly among the groups of four warps.
         constexpr int kParts = 16 / Roles<N>::unpacking;
-        const int wr = warp & 3, part0 = kParts == 1 ? (warp - 8) >> 2 : 0;
+        const int wr = warp & 3, part0 = ((warp - adding) >> 2) * kParts;
         const Unpack<X> unpack;
         const unsigned own0 = stage0 + x_bytes + wr * 1024 + lane * 16;
         unsigned full = bars, own = own0, phase = 0, a_phase[2] = {1, 1};
@@ -287,7 +294,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
                                 p[r][(half * 4 + i) * 2] = unpack.value(half ? w[r].z : w[r].x, i);
                                 p[r][(half * 4 + i) * 2 + 1] = unpack.value(half ? w[r].w : w[r].y, i);
                             }
-                    const int which = kParts == 1 ? 0 : q >> 1;
+                    const int which = q >> 1;
                     barrier_wait(half_bars + kAEmpty, a_phase[which], dead);
                     __syncwarp();
                     if (kParts == 1 || wg == 1) a_phase[which] ^= 1;
@@ -308,8 +315,10 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
     } else {
         // ---------------------------------------------------------------------------------------- a thread for every row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles<N>::add_regs));
-        const int wg = warp >> 2, wr = warp & 3, r16 = lane >> 4, in16 = lane & 15;
-        const unsigned d0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + 64, half_bars = bars + kHalf0 + wg * kHalf;
+        // (with sixteen warps, each has half of the hidden states)
+        constexpr int kOwn = N * 8 / adding;
+        const int wg = warp >> 2 & 1, columns = (warp >> 3) * kOwn, wr = warp & 3, r16 = lane >> 4, in16 = lane & 15;
+        const unsigned d0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + 64 + columns, half_bars = bars + kHalf0 + wg * kHalf;
         const bool bf16_scales = a.scale_type == FSB_BF16;
         // the scales of this row and of the other one that its words hold, for the two blocks of a chunk; fetched a chunk ahead
         const int64_t unit_s = (int64_t)scale_blocks(a.n_hidden, 32 * GS) * 8 * scale_bytes(32 * GS);
@@ -326,11 +335,11 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
             }
             next += kWords * kStep;
         };
-        u64 acc[N / 2];
+        u64 acc[kOwn / 2];
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) acc[i] = 0ull;
+        for (int i = 0; i < kOwn / 2; ++i) acc[i] = 0ull;
         unsigned slot = 0, d_phase = 0;
-        constexpr int kCols = N == 64 ? 64 : 32;     // taken out at a time
+        constexpr int kCols = kOwn == 64 ? 64 : kOwn < 32 ? 16 : 32;     // taken out at a time
         fetch(blocks > 1);
         for (int u = 0; u < mine; ++u) {
             for (int c = 0; c < chunks; ++c) {
@@ -356,11 +365,11 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
                     u64 s2;
                     asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(scale[e]));
 #pragma unroll
-                    for (int c0 = 0; c0 < N; c0 += kCols) {
+                    for (int c0 = 0; c0 < kOwn; c0 += kCols) {
                         uint32_t v[kCols];
                         const unsigned from = d0 + slot * N + c0;
-                        constexpr int kLast = N % kCols ? N % kCols : kCols;     // columns of the last turn (16 or 32)
-                        const bool last = c0 + kCols >= N;
+                        constexpr int kLast = kOwn % kCols ? kOwn % kCols : kCols;     // columns of the last turn (16 or 32)
+                        const bool last = c0 + kCols >= kOwn;
                         if (last && kLast == 16) tc_load16(from, v);
                         else {
 #pragma unroll
@@ -369,7 +378,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
                         tc_loaded();
 #pragma unroll
                         for (int i = 0; i < kCols; i += 16)
-                            if (c0 + i < N) tc_use(v + i);
+                            if (c0 + i < kOwn) tc_use(v + i);
                         if (last) {   // the columns may be written again
                             tc_before_sync();
                             __syncwarp();
@@ -377,7 +386,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
                         }
 #pragma unroll
                         for (int i = 0; i < kCols / 2; ++i)
-                            if (c0 + 2 * i < N) add_scaled(acc[c0 / 2 + i < N / 2 ? c0 / 2 + i : 0], s2, v[2 * i], v[2 * i + 1]);
+                            if (c0 + 2 * i < kOwn) add_scaled(acc[c0 / 2 + i < kOwn / 2 ? c0 / 2 + i : 0], s2, v[2 * i], v[2 * i + 1]);
                     }
                     slot = slot + 1 == slots ? 0 : slot + 1;
                     d_phase ^= slot == 0;
@@ -385,14 +394,14 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
             }
             if (__any_sync(0xffffffffu, *dead)) break;
             const int row = ((int)blockIdx.x + u * (int)gridDim.x) * kRows + wg * 128 + wr * 32 + lane;
-            float* to = a.logits + (int64_t)m0 * a.ld + row;
+            float* to = a.logits + (int64_t)(m0 + columns) * a.ld + row;
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
+            for (int i = 0; i < kOwn / 2; ++i) {
                 float lo, hi;
                 asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[i]));
                 if (row < a.n_vocab) {
-                    if (2 * i < mt) to[(int64_t)(2 * i) * a.ld] = lo;
-                    if (2 * i + 1 < mt) to[(int64_t)(2 * i + 1) * a.ld] = hi;
+                    if (columns + 2 * i < mt) to[(int64_t)(2 * i) * a.ld] = lo;
+                    if (columns + 2 * i + 1 < mt) to[(int64_t)(2 * i + 1) * a.ld] = hi;
                 }
                 acc[i] = 0ull;
             }
@@ -400,7 +409,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
         tc_before_sync();
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == others) {
         tc_after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
