@@ -88,6 +88,7 @@ struct fsb_head {
     int n_vocab = 0, n_hidden = 0, group = 0, scale_type = 0;
     unsigned char* d_weights = nullptr;
     unsigned char* d_scales = nullptr;
+    unsigned char* d_hidden = nullptr;   // room for the engine's most rows of hidden states
 };
 
 struct fsb_handle {

@@ -352,7 +352,7 @@ int launch_head(const HeadArgs& a, void* stream, int* launches) {
     // More hidden states than eight (groups of 32: than sixteen, since every group's sums have to be taken out of tensor memory) are the
     // other kernel's.  us here and there, 16 x 65536 x 1024 (32) 18.2, 19.2; 16 x 262144 x 2560 (32) 121, 133, (128) 98, 87; 9 of them
     // (32) 113, 132, (128) 92, 85; 9 x 65536 x 2048 (64) 25.9, 26.0; eight of them run here in 19.8 (32).
-    if (a.n_rows > (a.group == 32 ? 16 : 8) && launch_head_many(a, stream, &error)) return error;
+    if (a.n_rows > (a.group == 32 ? 16 : 8) && launch_head_many(a, stream, &error, launches)) return error;
     HeadPlan p{};
     p.a = a;
     p.vec = reinterpret_cast<uintptr_t>(a.hidden) % 16 == 0 && a.ld_hidden % 8 == 0;

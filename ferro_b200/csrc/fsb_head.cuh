@@ -46,9 +46,9 @@ struct Unpack {
     }
 };
 
-// Launches the kernel for more rows than tensor cores of a warp are good for; false if its operands cannot be (hidden states off 16-byte
-// boundaries).  `error`: a cudaError_t as int.
-bool launch_head_many(const HeadArgs& a, void* stream, int* error);
+// Launches the kernel for more rows than tensor cores of a warp are good for, and counts its launches; false if it cannot be (hidden states
+// off 16-byte boundaries, and no room to copy them to).  `error`: a cudaError_t as int.
+bool launch_head_many(const HeadArgs& a, void* stream, int* error, int* launches);
 int prepare_head_many();
 
 }  // namespace fsb

@@ -61,11 +61,16 @@ __device__ __forceinline__ bool barrier_passed(unsigned bar, unsigned parity) {
 }
 // Waits for the phase of this parity to end.  Gives up after a million looks (a second or so), or when somebody else of the CTA has:
 // `dead` is then set, what is computed from there on is nothing, and everybody leaves at the next unit.
-__device__ __forceinline__ void barrier_wait(unsigned bar, unsigned parity, volatile int* dead) {
+__device__ __forceinline__ void barrier_wait(unsigned bar, unsigned parity, volatile int* dead, int looks = FSB_INBOX_LOOKS) {
     if (barrier_passed(bar, parity)) return;
-    for (int i = 0, looks = FSB_INBOX_LOOKS; i < looks; ++i)
+    for (int i = 0; i < looks; ++i)
         if (barrier_passed(bar, parity) || *dead) return;
     *dead = 1;
+}
+// For what has been started and will end by itself, before its memory is left.
+__device__ __forceinline__ void barrier_outlast(unsigned bar, unsigned parity) {
+    int never = 0;
+    barrier_wait(bar, parity, &never, 1 << 20);
 }
 
 // One thread of the warp.  (With any other choice of one the compiler does not know that there is one, and has the instructions that take
@@ -206,8 +211,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
                 for (int i = 0; i < issued; ++i) {
                     if (full == bars) full = bars_end, phase ^= 1;
                     full -= 8;
-                    int never = 0;
-                    barrier_wait(full, phase ^ 1, &never);
+                    barrier_outlast(full, phase ^ 1);
                 }
         } else if (warp < others + 2) {
             // ------------------------------------------------------------------------------------ products of half `wg`
@@ -255,8 +259,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
                     }
                 // what has been issued is complete before anybody frees its memory
                 tc_commit(half_bars + kDone);
-                int never = 0;
-                barrier_wait(half_bars + kDone, 0, &never);
+                barrier_outlast(half_bars + kDone, 0);
             }
             __syncwarp();
         }
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles<N>::add_regs));
         // (with sixteen warps, each has half of the hidden states)
         constexpr int kOwn = N * 8 / adding;
-        const int wg = warp >> 2 & 1, columns = (warp >> 3) * kOwn, wr = warp & 3, r16 = lane >> 4, in16 = lane & 15;
+        const int wg = warp >> 2 & 1, columns = adding == 16 ? (warp >> 3) * kOwn : 0, wr = warp & 3, r16 = lane >> 4, in16 = lane & 15;
         const unsigned d0 = tmem + ((unsigned)(wr * 32) << 16) + wg * 256 + 64 + columns, half_bars = bars + kHalf0 + wg * kHalf;
         const bool bf16_scales = a.scale_type == FSB_BF16;
         // the scales of this row and of the other one that its words hold, for the two blocks of a chunk; fetched a chunk ahead
@@ -419,6 +422,19 @@ __global__ void __launch_bounds__(Roles<N>::threads, 1) head_many_kernel(const _
     }
 }
 
+// Hidden states off 16-byte boundaries, copied to where they lie one behind the other.
+__global__ void __launch_bounds__(256) pack_kernel(const unsigned short* hidden, int64_t ld, int n_rows, int n_hidden, uint4* out) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const int i = (int)(blockIdx.x * 256 + threadIdx.x), eights = n_hidden / 8, row = i / eights;
+    if (row >= n_rows) return;
+    const unsigned short* p = hidden + row * ld + (int64_t)(i - row * eights) * 8;
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (uint32_t)p[2 * j] | (uint32_t)p[2 * j + 1] << 16;
+    out[i] = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
@@ -473,13 +489,24 @@ int prepare_head_many() {
     return e ? e : prepare_type<__half>();
 }
 
-bool launch_head_many(const HeadArgs& a, void* stream, int* error) {
-    // tensor copies want rows on 16-byte boundaries
-    if (reinterpret_cast<uintptr_t>(a.hidden) % 16 != 0 || a.ld_hidden % 8 != 0) return false;
+bool launch_head_many(const HeadArgs& args, void* stream, int* error, int* launches) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return false;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
     ManyPlan p{};
-    p.a = a;
+    p.a = args;
+    HeadArgs& a = p.a;
+    // tensor copies want rows on 16-byte boundaries
+    if (reinterpret_cast<uintptr_t>(a.hidden) % 16 != 0 || a.ld_hidden % 8 != 0) {
+        if (a.n_rows > a.scratch_rows) return false;
+        const int threads = a.n_rows * (a.n_hidden / 8);
+        *error = launch_chained(pack_kernel, dim3((unsigned)((threads + 255) / 256)), 256, 0, s, a.chained != 0, static_cast<const unsigned short*>(a.hidden), a.ld_hidden, a.n_rows,
+                                a.n_hidden, static_cast<uint4*>(a.scratch));
+        if (*error != 0) return true;
+        ++*launches;
+        a.hidden = a.scratch;
+        a.ld_hidden = a.n_hidden;
+    }
     const int passes = (a.n_rows + kTokensMax - 1) / kTokensMax;
     p.tokens = (a.n_rows + passes - 1) / passes;
     CUtensorMap map;
@@ -488,7 +515,6 @@ bool launch_head_many(const HeadArgs& a, void* stream, int* error) {
     if (encode(&map, a.hidden_type == FSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.hidden), dims, strides, box, step,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     *error = a.hidden_type == FSB_BF16 ? run_group<__nv_bfloat16>(p, map, s) : run_group<__half>(p, map, s);
     return true;
 }

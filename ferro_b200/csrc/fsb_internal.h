@@ -179,6 +179,8 @@ struct HeadArgs {
     int32_t scale_type, hidden_type;
     int32_t sms;
     int32_t chained;           // as in AdjustArgs
+    int32_t scratch_rows;      // rows of n_hidden that fit `scratch` (0: not to be used)
+    void* scratch;
     uint32_t* late;            // a pinned host word that is set if a wait inside the kernel ran out
 };
 int prepare_head_kernels();   // for the current device, before its first launch_head

@@ -256,7 +256,10 @@ int queue_head(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidd
     a.hidden_type = hidden_type;
     a.sms = h->sm_count;
     a.late = h->h_empty_dev + 1;
+    // a captured launch may be replayed beside another one: it gets no memory that they would share
     a.chained = is_capturing(h) ? 0 : 1;
+    a.scratch = head->d_hidden;
+    a.scratch_rows = a.chained ? h->max_rows : 0;
     int launches = 0;
     const int e = launch_head(a, h->stream, &launches);
     h->counters.kernel_launches += (uint64_t)launches;
@@ -287,6 +290,7 @@ int create_head(fsb_handle* h, int n_vocab, int n_hidden, int group, const uint8
     unsigned char *tmp_w = nullptr, *tmp_s = nullptr;
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&head->d_weights), (size_t)head_weight_bytes(n_vocab, n_hidden));
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&head->d_scales), (size_t)head_scale_bytes(n_vocab, n_hidden, group));
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&head->d_hidden), (size_t)h->max_rows * (size_t)n_hidden * 2);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();   // whatever stream the weights were written on
     if (e == cudaSuccess && (flags & FSB_WEIGHTS_ON_HOST)) {
         e = cudaMalloc(reinterpret_cast<void**>(&tmp_w), wb);

@@ -564,6 +564,7 @@ int run_staged(fsb_handle* h, fsb_batch* b, const float* logits, unsigned flags,
 void release_head(fsb_head* head) {
     if (head->d_weights) cudaFree(head->d_weights);
     if (head->d_scales) cudaFree(head->d_scales);
+    if (head->d_hidden) cudaFree(head->d_hidden);
     delete head;
 }
 

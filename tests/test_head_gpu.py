@@ -61,6 +61,15 @@ def integers(rng, rows, V, K, group, scale_t, hidden_t):
     (300, 450, 640, 128, "bf16", "bf16", 0, 5),
     (4, 20000, 96, 32, "f16", "bf16", 0, 0),
     (40, 20000, 64, 64, "f16", "bf16", 0, 0),
+    (10, 700, 1280, 128, "bf16", "f16", 0, 0),
+    (12, 2050, 448, 64, "f16", "bf16", 1, 0),
+    (33, 777, 1056, 32, "bf16", "bf16", 1, 0),
+    (64, 1025, 2048, 64, "f16", "f16", 3, 2),
+    (97, 300, 896, 128, "f16", "bf16", 8, 0),
+    (144, 513, 1024, 32, "f16", "bf16", 0, 0),
+    (145, 600, 576, 64, "bf16", "f16", 0, 0),
+    (64, 40000, 96, 32, "f16", "bf16", 0, 0),
+    (65, 77777, 32, 32, "f16", "bf16", 0, 0),
 ])
 def test_exact_sums_are_exact(rows, V, K, group, scale_t, hidden_t, pad, out_pad):
     rng = np.random.default_rng(rows * 1000 + K)
@@ -146,10 +155,12 @@ def test_weights_may_come_from_the_host_and_go_away():
     other.free()      # (the engine has freed it)
 
 
-@pytest.mark.parametrize("rows", [2, 16, 70])
-def test_captured_and_replayed(rows):
+@pytest.mark.parametrize("rows,pad", [(2, 0), (16, 0), (70, 0), (70, 1), (140, 0)])
+def test_captured_and_replayed(rows, pad):
     rng = np.random.default_rng(6)
-    w, s, x = integers(rng, rows, 3000, 512, 64, "f16", "bf16")
+    w, s, x = integers(rng, rows, 3000, 512 + 64 * pad, 64, "f16", "bf16")
+    w, s, x = w[:, :256].contiguous(), s[:, :8].contiguous(), x[:, :512]     # (with a pad, rows off 16-byte boundaries)
+    x = torch.nn.functional.pad(x, (0, pad))
     e = engine()
     head = e.load_head(w, s)
     outs = [torch.zeros(rows, 3000, device="cuda") for _ in range(2)]
@@ -160,19 +171,42 @@ def test_captured_and_replayed(rows):
         g = torch.cuda.CUDAGraph()
         e.set_cuda_stream(streams[k].cuda_stream)
         with torch.cuda.graph(g, stream=streams[k]):
-            head.logits(xs[k], outs[k])
+            head.logits(xs[k][:, :512], outs[k])
         graphs.append(g)
     torch.cuda.synchronize()
     for _ in range(3):
         for k in range(2):
-            xs[k].copy_(torch.from_numpy(rng.integers(-7, 8, (rows, 512)).astype(np.float32)).cuda())
+            xs[k][:, :512].copy_(torch.from_numpy(rng.integers(-7, 8, (rows, 512)).astype(np.float32)).cuda())
         torch.cuda.synchronize()
         for k in range(2):            # at the same time
             with torch.cuda.stream(streams[k]):
                 graphs[k].replay()
         torch.cuda.synchronize()
         for k in range(2):
-            assert torch.equal(outs[k].double(), plain(w, s, xs[k]))
+            assert torch.equal(outs[k].double(), plain(w, s, xs[k][:, :512]))
+    e.close()
+
+
+@pytest.mark.parametrize("rows,pad", [(3, 0), (16, 1), (40, 0), (40, 1), (140, 0)])
+def test_queued_calls_read_their_own_hidden_states(rows, pad):
+    """Calls queued one behind the other, hidden states that change between them, other work in front: each is placed while the one
+    before it ends, and must not run ahead of it."""
+    rng = np.random.default_rng(rows)
+    w, s, _ = integers(rng, rows, 9000, 256, 32, "f16", "bf16")
+    e = engine()
+    head = e.load_head(w, s)
+    xs = [torch.from_numpy(rng.integers(-7, 8, (rows, 256 + pad)).astype(np.float32)).to(torch.bfloat16).cuda() for _ in range(8)]
+    big = torch.zeros(1 << 26, device="cuda")
+    x, outs = torch.zeros_like(xs[0]), [torch.zeros(rows, 9000, device="cuda") for _ in range(8)]
+    for k in range(8):
+        big.add_(1.0)                     # what comes before takes its time
+        x.copy_(xs[k])
+        head.logits(x[:, :256], outs[k])
+        if k % 2:
+            head.logits(x[:, :256], outs[k])
+    torch.cuda.synchronize()
+    for k in range(8):
+        assert torch.equal(outs[k].double(), plain(w, s, xs[k][:, :256])), k
     e.close()
 
 
