@@ -20,7 +20,7 @@ namespace {
 // of four), and the registers of the three kinds: a register per hidden state is what the first kind has.
 template <int ADD, int UNPACK, int LAUNCH_REGS, int ADD_REGS, int UNPACK_REGS, int OTHER_REGS>
 struct Split {
-    static constexpr int adding = ADD, unpacking = UNPACK, threads = 32 * (ADD + UNPACK + 4), add_regs = ADD_REGS, unpack_regs = UNPACK_REGS, other_regs = OTHER_REGS;
+    static constexpr int adding = ADD, unpacking = UNPACK, threads = 32 * (ADD + UNPACK + 4), launch_regs = LAUNCH_REGS, add_regs = ADD_REGS, unpack_regs = UNPACK_REGS, other_regs = OTHER_REGS;
     static_assert(32 * ADD * ADD_REGS + 32 * UNPACK * UNPACK_REGS + 128 * OTHER_REGS <= threads * LAUNCH_REGS, "a split of more registers than the launch has waits for ever");
 };
 // For 64 and 96 hidden states eight warps take out as much as sixteen with half of the columns each, in fewer instructions (64 and 96 x
@@ -467,13 +467,21 @@ int run_group(const ManyPlan& p, const CUtensorMap& map, cudaStream_t stream) {
     return p.a.group == 32 ? run_columns<X, 1>(p, map, stream) : p.a.group == 64 ? run_columns<X, 2>(p, map, stream) : run_columns<X, 4>(p, map, stream);
 }
 
+// The kernel shares out the registers that Split says it is launched with: it has to have been compiled for them.
+template <class X, int GS, int N>
+int prepare() {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, head_many_kernel<X, GS, N>);
+    if (e == cudaSuccess && at.numRegs < Roles<N>::launch_regs) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
+    return (int)e;
+}
 template <class X, int GS>
 int prepare_columns() {
-    cudaError_t e = cudaFuncSetAttribute(head_many_kernel<X, GS, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, 96>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(head_many_kernel<X, GS, 144>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024);
-    return (int)e;
+    int e = prepare<X, GS, 32>();
+    if (e == 0) e = prepare<X, GS, 64>();
+    if (e == 0) e = prepare<X, GS, 96>();
+    return e ? e : prepare<X, GS, 144>();
 }
 template <class X>
 int prepare_type() {
