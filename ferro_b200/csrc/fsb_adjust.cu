@@ -2,7 +2,7 @@
 // penalty over the penalty window, biases, grammar masks; from fp32, bf16 or fp16 logits to the rows that are sampled.
 //
 // Per row and column v, c(v) = occurrences of v in the row's window:
-//     x = cap * tanhf(x / cap);  c(v) > 0: x = (x > 0 ? x / p : x * p) - (f * c(v) + q);  x += bias(v);  masked: x = -inf
+//     x = cap * tanh(x / cap);  c(v) > 0: x = (x > 0 ? x / p : x * p) - (f * c(v) + q);  x += bias(v);  masked: x = -inf
 // in fp32, rounded once when it is stored.
 //
 // One pass over the logits, bound by its bytes.  A CTA takes a tile of one row, batch by batch of 16 columns a thread.  A batch's

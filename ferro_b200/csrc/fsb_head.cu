@@ -107,6 +107,7 @@ __device__ __forceinline__ float sum_of(uint32_t pair) {
 template <class X, int GS, int NT, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps, 1) head_kernel(const __grid_constant__ HeadPlan P) {
     constexpr int kThreads = 32 * kWarps, kAhead = Shape<kWarps>::ahead;
+    static_assert(kAhead % 2 == 0, "groups of 128 begin with an even block");
     extern __shared__ __align__(16) unsigned char smem[];
     const HeadArgs& a = P.a;
     constexpr int kBuffers = 2;
