@@ -86,8 +86,9 @@ struct Raw {
 };
 
 // cap * tanh(v / cap), inv = 1 / cap.  The division: a product and one correction by its exact remainder.  tanh a = 1 - 2 / (e^2a + 1), and
-// the first terms of its Taylor series where that would cancel (below 0.35 the next one is less than 2^-26 of the sum): within 2^-21
-// relative, as good as tanhf in half the instructions, of which a row of soft-capped fp32 logits is made (64 x 262144: 43 -> 40 us, 33 with eight columns a vector).
+// the first terms of its Taylor series where that would cancel (below 0.35 the next one is less than 2^-26 of the sum): within 2^-21 of the
+// cap and 2^-20 relative (at 0.35, where the errors of e^2a, the reciprocal and their sum count twice), in half of tanhf's instructions,
+// which is what a row of soft-capped fp32 logits costs (64 x 262144: 43 -> 40 us, 33 with eight columns a vector).
 __device__ __forceinline__ float capped(float v, float cap, float inv) {
     // from ten caps on tanh is 1 in fp32 (and infinity would have no remainder); NaN stays
     float x;

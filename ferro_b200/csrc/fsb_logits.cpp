@@ -59,6 +59,15 @@ int check_rows(fsb_handle* h, const void* p, int type, int64_t ld, int n_vocab, 
     return FSB_OK;
 }
 
+// What the adjustment kernel computes with: token ids are 32-bit, and a softcap leaves room for x / cap and its remainder on both sides
+// (at 1e38, ten caps are infinite; at 1e-45, 1 / cap is).
+int check_adjustable(fsb_handle* h, int n_vocab) {
+    if (h->softcap > 0.0f && !(h->softcap >= 1e-12f && h->softcap <= 1e12f))
+        return fail(h, FSB_ERR_RANGE, "a softcap of %g: logits are adjusted with one between 1e-12 and 1e12", (double)h->softcap);
+    if ((int64_t)h->vocab_offset + n_vocab > INT32_MAX) return fail(h, FSB_ERR_RANGE, "%d columns from token %d on: ids have 32 bits", n_vocab, h->vocab_offset);
+    return FSB_OK;
+}
+
 // Whether two matrices' address ranges intersect.
 bool overlap(const void* a, int64_t ld_a, int cols_a, size_t size_a, const void* b, int64_t ld_b, int cols_b, size_t size_b, int rows) {
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
@@ -382,6 +391,7 @@ int fsb_adjust_logits(fsb_handle* h, int n_rows, const int* stream_ids, const vo
         const bool in_place = out == logits && out_type == logits_type && out_ld == ld;
         if (rc == FSB_OK && !in_place && overlap(logits, ld, n_vocab, type_size(logits_type), out, out_ld, n_vocab, type_size(out_type), n_rows))
             rc = fail(h, FSB_ERR_INVALID, "out overlaps the logits");
+        if (rc == FSB_OK) rc = check_adjustable(h, n_vocab);
         if (rc == FSB_OK) rc = check_masks(h, m, n_rows, n_vocab);
         if (rc == FSB_OK) rc = check_streams(h, n_rows, stream_ids, false);
         if (rc) return rc;
@@ -401,6 +411,7 @@ int fsb_sample_batch_adjusted(fsb_handle* h, int n_rows, const int* stream_ids, 
         cudaSetDevice(h->device);
         int rc = check_common(h, n_rows, ld, n_vocab, h->own);
         if (rc == FSB_OK) rc = check_rows(h, logits, logits_type, ld, n_vocab, "logits");
+        if (rc == FSB_OK) rc = check_adjustable(h, n_vocab);
         if (rc == FSB_OK) rc = check_masks(h, m, n_rows, n_vocab);
         if (rc == FSB_OK) rc = check_streams(h, n_rows, stream_ids, true);
         if (rc == FSB_OK) rc = check_sampling(h, tokens_out, flags);
@@ -459,16 +470,17 @@ int fsb_sample_hidden(fsb_handle* h, const fsb_head* head, int n_rows, const int
         if (rc) return rc;
         const int V = head->n_vocab;
         const int64_t ld = stage_ld(h, n_rows, V);
-        rc = sync_streams(h, n_rows, stream_ids, (flags & FSB_APPEND_SAMPLED) != 0);
-        if (rc) return rc;
-        rc = queue_head(h, head, n_rows, hidden, hidden_type, ld_hidden, h->d_logits_stage, ld);
-        if (rc) return rc;
+        // (where there is nothing that the sampling kernels do not know, they apply the repetition penalty and the softcap themselves)
         bool adjusted = masks != nullptr;
         for (int i = 0; i < n_rows && !adjusted; ++i) {
             const Stream* s = get_stream(h, stream_ids[i]);
             adjusted = s->frequency != 0.0f || s->presence != 0.0f || s->n_bias > 0;
         }
-        // (where there is nothing that the sampling kernels do not know, they apply the repetition penalty and the softcap themselves)
+        if (adjusted) rc = check_adjustable(h, V);
+        if (rc == FSB_OK) rc = sync_streams(h, n_rows, stream_ids, (flags & FSB_APPEND_SAMPLED) != 0);
+        if (rc) return rc;
+        rc = queue_head(h, head, n_rows, hidden, hidden_type, ld_hidden, h->d_logits_stage, ld);
+        if (rc) return rc;
         if (adjusted) rc = queue_adjust(h, n_rows, stream_ids, h->d_logits_stage, FSB_F32, ld, V, m, h->d_logits_stage, FSB_F32, ld, true);
         if (rc) return rc;
         return sample_staged(h, n_rows, stream_ids, ld, V, adjusted, tokens_out, flags);

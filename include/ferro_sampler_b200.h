@@ -305,7 +305,8 @@ FSB_API int fsb_stream_bias_set(fsb_handle* h, int stream_id, const int32_t* ids
  * `out` ([n_rows][out_ld]; fp32, or the type of the logits).  With c(v) the number of times token v stands in the stream's
  * penalty window - its resident history (fsb_stream_history_*) cut by repeat_last_n and penalty_from, as for the repetition
  * penalty, src/sampler.cpp:11-14 -, for every column in this order, in fp32 and rounded once at the end:
- *     x = cap * tanh(x / cap)                     if the engine has a softcap (fsb_set_softcap)
+ *     x = cap * tanh(x / cap)                     if the engine has a softcap (fsb_set_softcap; here one between 1e-12 and 1e12,
+ *                                                 else FSB_ERR_RANGE), within 2^-20 relative
  *     x = x > 0 ? x / repetition : x * repetition     if c(v) > 0                                (src/sampler.cpp:17)
  *     x = x - (frequency * c(v) + presence)       if c(v) > 0
  *     x = x + bias(v)

@@ -354,12 +354,39 @@ int refusals() {
     fsb_destroy(s.h);    // (frees both heads)
     return 0;
 }
+
+// Settings of the engine that an adjustment cannot compute with, and what does not need one is sampled all the same.
+int ranges() {
+    Setup s(2);
+    int32_t tok[2];
+    fsb_head* head = nullptr;
+    WANT("create", fsb_head_create(s.h, 1000, 64, 32, weights_, scales_, FSB_F16, 0, &head), FSB_OK);
+    auto sampled = [&] { return fsb_sample_batch_adjusted(s.h, 2, s.sid.data(), rows_, FSB_F32, 1000, 1000, nullptr, 0, 0, nullptr, tok, 0); };
+    auto hidden = [&](const uint32_t* masks) { return fsb_sample_hidden(s.h, head, 2, s.sid.data(), hidden_, FSB_BF16, 64, masks, 1 << 27, 2, nullptr, tok, 0); };
+    for (float cap : {1e38f, 1e13f, 1e-13f, 1e-45f}) {
+        fsb_set_softcap(s.h, cap);
+        WANT("adjust", adjust(s, 2), FSB_ERR_RANGE);
+        WANT("sample", sampled(), FSB_ERR_RANGE);
+        WANT("masked", hidden(masks_), FSB_ERR_RANGE);
+        WANT("plain", hidden(nullptr), FSB_OK);
+    }
+    for (float cap : {1e12f, 30.0f, 1e-12f, 0.0f}) {
+        fsb_set_softcap(s.h, cap);
+        WANT("adjust", adjust(s, 2), FSB_OK);
+    }
+    for (int32_t past : {0, 1, 1000}) {
+        fsb_set_vocab_offset(s.h, INT32_MAX - 1000 + past);
+        WANT("offset", adjust(s, 2), past ? FSB_ERR_RANGE : FSB_OK);
+        if (past) WANT("offset", hidden(masks_), FSB_ERR_RANGE);
+    }
+    return 0;
+}
 }  // namespace
 
 int main(int argc, char** argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     const int rc = what == "settings" ? settings() : what == "regions" ? regions() : what == "sampling" ? sampling() : what == "head" ? head()
-                   : what == "refusals" ? refusals() : 2;
+                   : what == "refusals" ? refusals() : what == "ranges" ? ranges() : 2;
     if (rc == 0) std::puts("ok");
     return rc;
 }

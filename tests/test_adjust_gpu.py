@@ -195,6 +195,45 @@ def test_special_values(in_t):
     eng.close()
 
 
+@pytest.mark.parametrize("cap", [1e-12, 0.5, 30.0, 1e12])
+def test_softcap_over_its_range(cap):
+    """Relative error: with a = 2 x / cap, e^a is within 2^-22 and its argument's rounding, the reciprocal within 2^-23; 2 / (e^a + 1) is 0.66 where the
+    result is smallest, 0.34: below 1.7 * 2^-21 with the sums' roundings, 2^-23 for the division and the product by cap: 2^-20 in all.  Quotients
+    below the smallest normal number are off by 2^-149."""
+    cap = float(np.float32(cap))
+    f = torch.finfo(torch.float32)
+    u = np.concatenate([np.linspace(-12, 12, 20001), np.linspace(-0.4, 0.4, 4001), 10.0 ** np.linspace(-30, 0, 61)]) * cap
+    vals = np.concatenate([u, [INF, -INF, float("nan"), 0.0, -0.0, f.max, f.min, f.tiny, -f.tiny, 1.0, -1.0]]).astype(np.float32)
+    logits = torch.from_numpy(vals[None]).cuda()
+    eng = engine_for(1, len(vals))
+    eng.set_softcap(cap)
+    sid = eng.open_stream(fb.make_params(1, repetition_penalty=1.0, seed=1))
+    got = eng.adjust_logits([sid], logits, torch.empty_like(logits)).cpu().numpy()[0].astype(np.float64)
+    want = cap * np.tanh(vals.astype(np.float64) / cap)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    worst = np.abs(got[ok] - want[ok]) - (2.0 ** -20 * np.abs(want[ok]) + 2.0 ** -149 * max(cap, 1.0))
+    assert worst.max() <= 0, vals[ok][np.argmax(worst)]
+    eng.close()
+
+
+@pytest.mark.parametrize("rows,in_t", [(1, "f32"), (3, "bf16")])
+def test_windows_of_more_than_65535_ids(rows, in_t):
+    """Counts that 16 bits do not hold, and windows whose ids fall into all tiles."""
+    rng = np.random.default_rng(12)
+    V, n = 20003, 70001
+    hists = [np.full(n, 7, dtype=np.int32), rng.integers(0, V, 65536).astype(np.int32), rng.integers(0, V, 65535).astype(np.int32)][:rows]
+    hists[0][-5:] = [7, V - 1, 7, 4096, 0]
+    logits = torch.from_numpy(rng.standard_normal((rows, V)).astype(np.float32) * 4).cuda().to(T[in_t])
+    rep, freq, pres, bias = [1.3] * rows, [0.001, 0.25, -0.5][:rows], [0.5] * rows, [{7: 2.0, V - 1: -1.0}] * rows
+    eng = engine_for(rows, V)
+    sids = open_rows(eng, rep, freq, pres, hists, bias)
+    want, mag = plain(logits, V, hists, rep, freq, pres, bias, [None] * rows, 0.0)
+    out = eng.adjust_logits(sids, logits, torch.empty(rows, V, device="cuda"))
+    check(out, want, mag, 0.0, "f32")
+    eng.close()
+
+
 @pytest.mark.parametrize("offset", [0, 1, 31, 32, 5000])
 def test_vocabulary_shards(offset):
     rng = np.random.default_rng(offset)
