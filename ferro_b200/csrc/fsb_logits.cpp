@@ -440,6 +440,7 @@ int fsb_head_free(fsb_handle* h, fsb_head* head) {
     if (!h) return FSB_ERR_INVALID;
     if (!owns(h, head)) return fail(h, FSB_ERR_INVALID, "not a head of this engine");
     cudaSetDevice(h->device);
+    if (is_capturing(h)) return fail(h, FSB_ERR_INVALID, "a head is not freed inside a stream capture");
     cudaStreamSynchronize(h->stream);
     h->heads.erase(std::find(h->heads.begin(), h->heads.end(), head));
     release_head(head);

@@ -336,7 +336,7 @@ FSB_API int fsb_sample_batch_adjusted(fsb_handle* h, int n_rows, const int* stre
  * device memory, or with FSB_WEIGHTS_ON_HOST in host memory.  fsb_head_create copies them into the layout that the kernels
  * read and waits for that; the caller's arrays are not needed afterwards.  It allocates device memory: n_hidden / 2 bytes a
  * row and the scales, rows rounded up to 256, and 2 * n_hidden bytes for each of the engine's max_rows.  A head belongs to the engine that created it and is freed with it at the
- * latest.  (The dequantisation of a Q4_0 block: 32 weights, d * (q - 8).)  No reference counterpart in this form: the
+ * latest (not inside a stream capture: FSB_ERR_INVALID; a graph that holds its launches must not be replayed afterwards).  (The dequantisation of a Q4_0 block: 32 weights, d * (q - 8).)  No reference counterpart in this form: the
  * reference's heads are Q8 (q8gemv). */
 typedef struct fsb_head fsb_head;
 #define FSB_WEIGHTS_ON_HOST 1u
@@ -348,7 +348,9 @@ FSB_API int fsb_head_free(fsb_handle* h, fsb_head* head);
  * not overlap.  Weights are not rounded, products are exact, sums and scales fp32.  Asynchronous on the engine's stream; may be
  * captured into a CUDA graph, and such launches share no workspace.  At most 65535 rows, however many the engine was created for.
  * Fastest where hidden states start on 16-byte boundaries (other ones are copied, if they are max_rows at most and not
- * captured).  FSB_ERR_DEVICE if a wait inside an earlier launch ran out: that one's logits are not complete. */
+ * captured).  A row of hidden states with an infinity or a NaN has no finite logits (NaN, it may be, where the formula
+ * has an infinity), nor need one with values beyond 2^115; the other rows are what they are without it.
+ * FSB_ERR_DEVICE if a wait inside an earlier launch ran out: that one's logits are not complete. */
 FSB_API int fsb_head_logits(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidden, int hidden_type, int64_t ld_hidden, float* logits,
                             int64_t ld);
 /* A decode step from hidden states to tokens: fsb_head_logits into the engine's own memory, then what

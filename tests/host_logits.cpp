@@ -355,6 +355,20 @@ int refusals() {
     return 0;
 }
 
+// A head that is let go while its engine's stream is being captured (by a garbage collector, say): the capture goes on, the head stays.
+int captured_free() {
+    Setup s(1);
+    fsb_head* head = nullptr;
+    WANT("create", fsb_head_create(s.h, 1000, 64, 32, weights_, scales_, FSB_F16, 0, &head), FSB_OK);
+    capturing_ = true;
+    const int rc = fsb_head_free(s.h, head), used = fsb_head_logits(s.h, head, 1, hidden_, FSB_BF16, 64, out_, 1000);
+    capturing_ = false;
+    WANT("captured", rc, FSB_ERR_INVALID);
+    WANT("still there", used, FSB_OK);
+    WANT("free", fsb_head_free(s.h, head), FSB_OK);
+    return 0;
+}
+
 // Settings of the engine that an adjustment cannot compute with, and what does not need one is sampled all the same.
 int ranges() {
     Setup s(2);
@@ -386,7 +400,7 @@ int ranges() {
 int main(int argc, char** argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     const int rc = what == "settings" ? settings() : what == "regions" ? regions() : what == "sampling" ? sampling() : what == "head" ? head()
-                   : what == "refusals" ? refusals() : what == "ranges" ? ranges() : 2;
+                   : what == "refusals" ? refusals() : what == "ranges" ? ranges() : what == "captured_free" ? captured_free() : 2;
     if (rc == 0) std::puts("ok");
     return rc;
 }
