@@ -88,6 +88,10 @@ int check_streams(fsb_handle* h, int n_rows, const int* stream_ids, bool once) {
     return FSB_OK;
 }
 
+// Whether a launch may be placed while the one before it ends.  Not in launch mode 1, whose sampling kernels read logits that are complete
+// before the kernel in front of them starts: kernels that start one inside the other would carry them past that.
+bool may_chain(const fsb_handle* h) { return h->launch_overlap != 1; }
+
 // Queues the adjustment of rows whose arguments have been checked and whose histories are on the device.
 int queue_adjust(fsb_handle* h, int n_rows, const int* stream_ids, const void* logits, int logits_type, int64_t ld, int n_vocab, const Masks& m, void* out,
                  int out_type, int64_t out_ld, bool report_empty) {
@@ -123,7 +127,7 @@ int queue_adjust(fsb_handle* h, int n_rows, const int* stream_ids, const void* l
     a.n_vocab = n_vocab;
     a.vocab_offset = h->vocab_offset;
     a.softcap = h->softcap;
-    a.chained = 1;
+    a.chained = may_chain(h);
     if (report_empty) *static_cast<volatile uint32_t*>(h->h_empty) = 0u;
     int launches = 0;
     const int e = launch_adjust(a, rows.data(), h->stream, &launches);
@@ -266,9 +270,10 @@ int queue_head(fsb_handle* h, const fsb_head* head, int n_rows, const void* hidd
     a.sms = h->sm_count;
     a.late = h->h_empty_dev + 1;
     // a captured launch may be replayed beside another one: it gets no memory that they would share
-    a.chained = is_capturing(h) ? 0 : 1;
+    const bool captured = is_capturing(h);
+    a.chained = !captured && may_chain(h);
     a.scratch = head->d_hidden;
-    a.scratch_rows = a.chained ? h->max_rows : 0;
+    a.scratch_rows = captured ? 0 : h->max_rows;
     int launches = 0;
     const int e = launch_head(a, h->stream, &launches);
     h->counters.kernel_launches += (uint64_t)launches;

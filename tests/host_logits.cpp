@@ -369,6 +369,21 @@ int captured_free() {
     return 0;
 }
 
+// Launch mode 1 reads logits that are complete before the kernel in front of it starts: our own kernels then start one behind the other.
+int modes() {
+    Setup s(2);
+    fsb_head* head = nullptr;
+    WANT("create", fsb_head_create(s.h, 1000, 64, 32, weights_, scales_, FSB_F16, 0, &head), FSB_OK);
+    for (int mode = 0; mode < 3; ++mode) {
+        fsb_set_launch_overlap(s.h, mode);
+        WANT("head", fsb_head_logits(s.h, head, 2, hidden_, FSB_BF16, 64, out_, 1000), FSB_OK);
+        WANT("adjust", adjust(s, 2), FSB_OK);
+        if (heads_.back().chained != (mode != 1) || heads_.back().scratch_rows != 2) return bad("head", mode, heads_.back().chained, mode != 1);
+        if (adjusted_.back()->a.chained != (mode != 1)) return bad("adjust", mode, adjusted_.back()->a.chained, mode != 1);
+    }
+    return 0;
+}
+
 // Settings of the engine that an adjustment cannot compute with, and what does not need one is sampled all the same.
 int ranges() {
     Setup s(2);
@@ -400,7 +415,7 @@ int ranges() {
 int main(int argc, char** argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     const int rc = what == "settings" ? settings() : what == "regions" ? regions() : what == "sampling" ? sampling() : what == "head" ? head()
-                   : what == "refusals" ? refusals() : what == "ranges" ? ranges() : what == "captured_free" ? captured_free() : 2;
+                   : what == "refusals" ? refusals() : what == "ranges" ? ranges() : what == "captured_free" ? captured_free() : what == "modes" ? modes() : 2;
     if (rc == 0) std::puts("ok");
     return rc;
 }

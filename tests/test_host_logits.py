@@ -24,7 +24,7 @@ def driver(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("what", ["settings", "regions", "sampling", "head", "refusals", "ranges", "captured_free"])
+@pytest.mark.parametrize("what", ["settings", "regions", "sampling", "head", "refusals", "ranges", "captured_free", "modes"])
 def test_host_logits(driver, what):
     env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0")
     r = subprocess.run([driver, what], capture_output=True, text=True, timeout=120, env=env)
