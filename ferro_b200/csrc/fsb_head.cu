@@ -2,7 +2,12 @@
 //
 // Weights are never rounded: a 4-bit weight becomes the 16-bit float 16 + q by one logic operation (its bits are the upper
 // mantissa bits of a number between 16 and 32), tensor cores add up (16 + q) x in fp32 for one group on top of -24 times the
-// group's sum of x, and the scale is multiplied in fp32.  For up to 16 hidden states a pass the weights' bytes bound it.
+// group's sum of x, and the scale is multiplied in fp32.
+//
+// head_kernel, here, is for up to 8 hidden states (16 with groups of 32); more are fsb_head_many.cu's.  Instructions on the logic pipe (68 % of
+// its rate in 1 x 262144 x 2560, groups of 128) bound it as much as the weights' bytes do, and the start and end of the launch where there
+// are few.  us, and the weights and scales read a second: 1 x 262144 x 2560 (128) 64, 5.4 TB/s; 8 x 65536 x 2048 (32) 19.7, 3.8; 5 x
+// 100003 x 2016 (32) 31.8, 3.6; 1 x 65536 x 1024 (32) 10.5, 3.6.
 //
 // Layout (laid out once): units of eight pairs of tiles of 16 vocabulary rows; of a unit block by block of 64 weights a row, pair by
 // pair, 16 bytes per tile and lane of the warp that multiplies it.  Lane 4 g + t holds, of rows g and g + 8 of the tile and of both halves
@@ -60,7 +65,7 @@ __global__ void layout_scales_kernel(const unsigned short* __restrict__ s, int n
     }
 }
 
-// ------------------------------------------------------------------------------------------------ up to 16 rows a pass
+// ------------------------------------------------------------------------------------------------ up to 16 hidden states a pass
 struct HeadPlan {
     HeadArgs a;
     int ksplit;        // warps that share a tile pair's k; the CTA's other warps take other tile pairs

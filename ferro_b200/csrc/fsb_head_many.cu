@@ -1,11 +1,18 @@
 // fsb_head_many.cu - the LM head (fsb_head.cu) for more hidden states than a warp's own tensor instructions are good for: tcgen05.mma with
-// the weights as operand A in tensor memory, unpacked there by the warps that later take the sums out again.
+// the weights as operand A in tensor memory.
 //
 // A CTA takes 256 vocabulary rows at a time, in two halves, and all hidden states of the pass (up to 144).  Warps have one part each:
 // some unpack weights (32 rows of a block of 64 weights at a time) to q - 8 in bf16 / fp16, which is exact, and store them to tensor
-// memory as 32 columns of pairs; two issue the products of 128 rows; eight take the sums of one group of weights out again, a thread
+// memory as 32 columns of pairs; two issue the products of 128 rows; others take the sums of one group of weights out again, a thread
 // for every row and a register for every hidden state, and add them up times the row's scale, two to an instruction; one has weights
-// and hidden states copied into a ring of stages of two blocks.
+// and hidden states copied into a ring of stages of two blocks.  A scale for every row and group cannot be part of a product whose
+// operands are exact in 16 bits, so sums leave tensor memory once a group.
+//
+// That bounds it: of 1270 cycles a block of 64 weights (64 hidden states, groups of 32) the warps that take out are busy 870, some 300 for
+// every piece that they load and wait for, and the unpacking ones wait 870.  us: 64 x 262144 x 2560, groups of 32 173 (2.57 TB/s, 495 TFLOP/s;
+// bytes alone 68), 32 hidden states 121; 136 x 65536 x 2048, groups of 64 56 (650 TFLOP/s; products alone 23), of 128 47.  Slower:
+// scales in the operand, as two numbers of five and six bits and twice the products, sums taken out once per 128 weights (203, unpacking
+// is then what it waits for); both halves of the rows one after the other over one ring of sums (68 for the 56, 48 for the 47).
 #include <cuda.h>
 
 #include <algorithm>
