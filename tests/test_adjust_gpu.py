@@ -234,6 +234,27 @@ def test_windows_of_more_than_65535_ids(rows, in_t):
     eng.close()
 
 
+@pytest.mark.parametrize("in_t,out_t", [("bf16", "f32"), ("f16", "f16")])
+def test_rows_that_are_gigabytes_apart(in_t, out_t):
+    """Row offsets beyond 2^31 elements, and masks beyond 2^31 words' bytes."""
+    rng = np.random.default_rng(15)
+    V, ld, rows = 5000, 1 << 30, 3
+    logits = torch.empty(2 * ld + V, dtype=T[in_t], device="cuda").as_strided((rows, V), (ld, 1))
+    logits.copy_(torch.from_numpy(rng.standard_normal((rows, V)).astype(np.float32) * 4))
+    out = torch.empty(2 * ld + V, dtype=T[out_t], device="cuda").as_strided((rows, V), (ld, 1))
+    allowed = [rng.random(V) < 0.5 for _ in range(rows)]
+    words = (V + 31) // 32
+    masks = torch.empty(ld + words, dtype=torch.int32, device="cuda").as_strided((rows, words), (ld // 2, 1))
+    masks.copy_(pack(allowed, words))
+    eng = engine_for(rows, V)
+    rep, freq, pres, hists, bias = settings(rng, rows, V, 400, 30)
+    sids = open_rows(eng, rep, freq, pres, hists, bias)
+    want, mag = plain(logits, V, hists, rep, freq, pres, bias, allowed, 0.0)
+    eng.adjust_logits(sids, logits, out, masks=masks)
+    check(out, want, mag, 0.0, out_t)
+    eng.close()
+
+
 @pytest.mark.parametrize("offset", [0, 1, 31, 32, 5000])
 def test_vocabulary_shards(offset):
     rng = np.random.default_rng(offset)

@@ -132,6 +132,25 @@ def test_infinite_and_nan_hidden_states_stay_in_their_rows():
         e.close()
 
 
+@pytest.mark.parametrize("rows", [2, 20])
+def test_weights_and_rows_beyond_four_gigabytes(rows):
+    """4.7 GB of weights, laid out and multiplied; hidden states and logits whose rows are gigabytes apart."""
+    V, K, group, ld = 575000, 16384, 128, (1 << 30) // 8
+    torch.manual_seed(rows)
+    w = torch.randint(0, 256, (V, K // 2), dtype=torch.uint8, device="cuda")
+    s = (2.0 ** torch.randint(-2, 2, (V, K // group), device="cuda")).to(torch.bfloat16)
+    x = torch.empty((rows - 1) * ld + K, dtype=torch.bfloat16, device="cuda").as_strided((rows, K), (ld, 1))
+    x.copy_(torch.randint(-7, 8, (rows, K), device="cuda"))
+    out = torch.empty((rows - 1) * ld + V, dtype=torch.float32, device="cuda").as_strided((rows, V), (ld, 1))
+    e = fb.Engine(device=0, max_rows=32, max_vocab=1 << 20, max_hist_ids=1 << 16)
+    e.set_cuda_stream(torch.cuda.current_stream().cuda_stream)
+    head = e.load_head(w, s)
+    head.logits(x, out)
+    for at in (0, 262100, 524200, V - 300):      # (2^32 bytes of weights end at row 524288)
+        assert torch.equal(out[:, at:at + 300].double(), plain(w[at:at + 300], s[at:at + 300], x)), at
+    e.close()
+
+
 def test_weights_may_come_from_the_host_and_go_away():
     rng = np.random.default_rng(4)
     w, s, x = integers(rng, 5, 777, 160, 32, "bf16", "f16")
