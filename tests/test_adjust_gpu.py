@@ -307,6 +307,38 @@ def test_settings_come_and_go_with_their_stream():
     eng.close()
 
 
+def test_settings_that_change_while_calls_are_queued():
+    """A call sees the settings of its moment, however late it runs: histories, biases and regions that change hands behind it."""
+    rng = np.random.default_rng(9)
+    V = 3000
+    logits = torch.from_numpy(rng.standard_normal((1, V)).astype(np.float32) * 3).cuda()
+    eng = engine_for(1, V, ids=2048)
+    big = torch.zeros(1 << 27, device="cuda")
+    outs, wants = [], []
+    torch.cuda.synchronize()
+    for _ in range(12):
+        big.add_(1.0)                                    # everything below is queued behind this
+        hist = rng.integers(0, 40, int(rng.integers(1, 500))).astype(np.int32)
+        bias = {int(i): 1.5 for i in rng.permutation(V)[: int(rng.integers(1, 200))]}
+        sid = int(open_rows(eng, [1.3], [0.25], [0.5], [hist], [bias])[0])
+        for step in range(3):
+            out = torch.empty_like(logits)
+            eng.adjust_logits([sid], logits, out)
+            outs.append(out)
+            wants.append(plain(logits, V, [hist], [1.3], [0.25], [0.5], [bias], [None], 0.0))
+            if step == 0:
+                bias = {int(i): -2.0 for i in rng.permutation(V)[:150]}
+                eng.set_bias(sid, bias)
+            else:
+                hist = rng.integers(0, 40, 300).astype(np.int32)
+                eng.history_set(sid, hist)
+        eng.close_stream(sid)                            # its regions are the next one's
+    torch.cuda.synchronize()
+    for out, (want, mag) in zip(outs, wants):
+        check(out, want, mag, 0.0, "f32")
+    eng.close()
+
+
 def test_one_stream_for_several_rows_and_another_cuda_stream():
     rng = np.random.default_rng(8)
     V, rows = 9000, 6
