@@ -461,7 +461,7 @@ template <class X, int GS, int N>
 int run(ManyPlan p, const CUtensorMap& map, cudaStream_t stream) {
     const int units = (p.a.n_vocab + kRows - 1) / kRows;
     const dim3 grid((unsigned)std::min(units, p.a.sms), (unsigned)((p.a.n_rows + p.tokens - 1) / p.tokens));
-    p.stages = std::min(kStagesMax, (kSharedMax - 3072) / stage_bytes<N>());
+    p.stages = std::min(kStagesMax, (kSharedMax - 3 * 1024) / stage_bytes<N>());
     return launch_chained(head_many_kernel<X, GS, N>, grid, Roles<N>::threads, (size_t)(p.stages * stage_bytes<N>() + 1024), stream, p.a.chained != 0, p, map);
 }
 template <class X, int GS>
